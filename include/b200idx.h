@@ -48,6 +48,8 @@ enum {
  *   F16: fp16 rows, fp32 accumulation (the reference's own Flat arithmetic,
  *        FR/ascend/impl/AscendIndexImpl.cpp:339-346). */
 enum { B200IDX_F32 = 0, B200IDX_F16 = 1 };
+/* Element type of rows in device memory that the operators below read or write, besides the two above. */
+enum { B200IDX_BF16 = 2 };
 
 /* ---- construction: AscendIndexFlat(int dims, MetricType, AscendIndexFlatConfig)
  *      FR/ascend/AscendIndexFlat.h:56; AscendIndexInt8Flat(...) FR/ascend/AscendIndexInt8Flat.h:63-64;
@@ -130,6 +132,57 @@ int b200idx_merge_topk_device(int nsrc, int64_t n, int k, int descending, const 
 int b200idx_merge_topk_device_strided(int nsrc, int64_t n, int k, int descending, const float* Din_dev,
                                       const int64_t* Iin_dev, int64_t src_stride_bytes, float* D_dev,
                                       int64_t* I_dev, void* stream);
+
+/* ---- operators on rows in few bits: what makes the rows of compressed exact indexes and scores them.
+ *      (The reference takes rows that are int8 or fp16 already; FR/ascend/AscendIndexInt8.h:70-84.)
+ *      All pointers are device pointers of ONE device, which need not be the current one, aligned to
+ *      their element type unless more is said; row strides (ld) count elements, 0 = rows without gaps.
+ *      Work is queued on `stream` (a cudaStream_t of that device, NULL = its default stream), nothing is
+ *      allocated or waited for, calls may overlap and may be captured into a graph.  Outputs must not
+ *      overlap inputs or one another except where it is allowed below.  0 < n < 1e9, 0 < d <= 16384; rows
+ *      behind n and elements behind d are neither read nor written (scales: see below).
+ *      Messages of failing calls: b200idx_last_error(NULL). ----
+ *
+ * Root-mean-square norm with the residual's addition, rounded to int8 rows with scales: the last step of an
+ * embedding model and what an Int8Flat index stores, in one pass.  Per row of x (type dtype: F32, F16, BF16)
+ *   s = x + residual            rounded to dtype and written to `sum` (residual NULL: s = x, sum must be NULL;
+ *                               sum may be x or residual itself, with the same stride)
+ *   y = s / sqrt(mean(s^2) + eps) * weight          weight[d] in dtype, 1e-12 <= eps <= 1
+ *   q = round(y / scale) to nearest, ties to even, cut to [-127, 127];  q has row stride ldq
+ *   scale: static_scale[0] where that is given, else max|y| / 127 of the row, written to scales[n]
+ * (exactly one of scales and static_scale is NULL).  A row of zeros has scale 0 and q 0.  A row with a NaN or
+ * an infinity has q 0 and scale NaN; a static scale that is not a positive number gives q 0. */
+int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64_t ldx, const void* residual,
+                               int64_t ldr, void* sum, int64_t lds, const void* weight, float eps,
+                               const float* static_scale, int8_t* q, int64_t ldq, float* scales, void* stream);
+/* The values that int8 rows stand for, out = q * scale in dtype (exactly one of scales, static_scale is NULL). */
+int b200idx_i8_dequantize_device(int64_t n, int d, const int8_t* q, int64_t ldq, const float* scales,
+                                 const float* static_scale, int dtype, void* out, int64_t ldo, void* stream);
+
+/* Microscaled 4-bit floating point ("MX4"): a row is cut into blocks of 32 elements; a block has one scale
+ * 2^e (a byte e + 127, 255 = NaN) and 32 codes of sign, 2 exponent bits and 1 mantissa bit that stand for
+ * 0, 0.5, 1, 1.5, 2, 3, 4, 6.  Rounding: e = floor(log2(max|v|)) - 2, at least -127; a code is the nearest
+ * to v / 2^e, ties to the even code, magnitudes above 6 become 6.  A block of zeros has scale byte 0; a
+ * block with a NaN or an infinity has scale byte 255 and codes 0 and stands for NaN.
+ * Layout, with nb = ceil(d / 32) and ng = ceil(nb / 4):
+ *   codes : n rows of b200idx_mx4_row_bytes(d) = 16 nb bytes, element 2 i in the low half of byte i, zeros
+ *           behind element d; 16-byte aligned
+ *   scales: b200idx_mx4_scale_bytes(n, d) = 512 ceil(n / 128) ng bytes, the order the tensor core reads: block
+ *           c of row r at (r / 128 * ng + c / 4) * 512 + r % 32 * 16 + r % 128 / 32 * 4 + c % 4; 16-byte
+ *           aligned.  A row's bytes of blocks nb .. 4 ng - 1 are written as 127; those of rows behind n are
+ *           left as they are and may hold anything. */
+int64_t b200idx_mx4_row_bytes(int d);
+int64_t b200idx_mx4_scale_bytes(int64_t n, int d);
+int b200idx_mx4_quantize_device(int64_t n, int d, int dtype, const void* x, int64_t ldx, uint8_t* codes,
+                                uint8_t* scales, void* stream);
+/* out = the values that the codes stand for, in dtype (F16 rounds and overflows to infinity; F32, BF16 exact). */
+int b200idx_mx4_dequantize_device(int64_t n, int d, const uint8_t* codes, const uint8_t* scales, int dtype,
+                                  void* out, int64_t ldo, void* stream);
+/* All scores of m rows a against n rows b: out[i][j] = sum_k a[i][k] b[j][k], added up in fp32 and rounded to
+ * dtype once.  0 < m, n < 1e9.  An output depends on its two rows alone; the order of its sum follows from m, n and d. */
+int b200idx_mx4_product_device(int64_t m, int64_t n, int d, const uint8_t* a_codes, const uint8_t* a_scales,
+                               const uint8_t* b_codes, const uint8_t* b_scales, int dtype, void* out, int64_t ldo,
+                               void* stream);
 
 /* ---- reset / remove_ids / bookkeeping: FR/ascend/AscendIndex.h:77,91;
  *      getBaseSize / getBase / getIdxMap FR/ascend/AscendIndexFlat.h:69-75,
@@ -226,7 +279,7 @@ int b200idx_set_timing(b200idx_t* h, int enabled);
 /* The cudaStream_t all of this index's kernels are launched on. */
 void* b200idx_stream(const b200idx_t* h);
 
-/* Message of the last failing call on this handle (h = NULL: last failing create). */
+/* Message of the last failing call on this handle (h = NULL: last failing create or operator). */
 const char* b200idx_last_error(const b200idx_t* h);
 /* The status code this library returns for an internal failure with the given message: a device-side
  * wait that ran out of its bound (the kernels give every mbarrier / flag wait a limit and report

@@ -20,6 +20,7 @@ METRIC_L2 = 1
 METRIC_INT8_COSINE = 2     # Int8Flat only: the reference's fp16 cosine (see include/b200idx.h)
 F32 = 0
 F16 = 1
+BF16 = 2                   # rows of the operators below only
 
 _lib = None
 
@@ -73,6 +74,13 @@ def load() -> C.CDLL:
         "b200idx_search_multi_stats": (i32, [i32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
         "b200idx_merge_topk_device": (i32, [i32, i64, i32, i32, vp, vp, vp, vp, vp]),
         "b200idx_merge_topk_device_strided": (i32, [i32, i64, i32, i32, vp, vp, i64, vp, vp, vp]),
+        "b200idx_rms_norm_i8_device": (i32, [i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, vp, i64, vp, vp]),
+        "b200idx_i8_dequantize_device": (i32, [i64, i32, vp, i64, vp, vp, i32, vp, i64, vp]),
+        "b200idx_mx4_row_bytes": (i64, [i32]),
+        "b200idx_mx4_scale_bytes": (i64, [i64, i32]),
+        "b200idx_mx4_quantize_device": (i32, [i64, i32, i32, vp, i64, vp, vp, vp]),
+        "b200idx_mx4_dequantize_device": (i32, [i64, i32, vp, vp, i32, vp, i64, vp]),
+        "b200idx_mx4_product_device": (i32, [i64, i64, i32, vp, vp, vp, vp, i32, vp, i64, vp]),
         "b200idx_reset": (i32, [vp]),
         "b200idx_remove_ids": (i32, [vp, i64, vp, C.POINTER(i64)]),
         "b200idx_ntotal": (i64, [vp]),
@@ -122,6 +130,8 @@ EXPORTED_SYMBOLS = [
     "b200idx_ivfpq_search_preassigned_device", "b200idx_ivfpq_get_nprobe", "b200idx_ivfpq_list_length",
     "b200idx_ivfpq_get_list", "b200idx_stats", "b200idx_set_timing", "b200idx_stream", "b200idx_last_error",
     "b200idx_status_of_message",
+    "b200idx_rms_norm_i8_device", "b200idx_i8_dequantize_device", "b200idx_mx4_row_bytes", "b200idx_mx4_scale_bytes",
+    "b200idx_mx4_quantize_device", "b200idx_mx4_dequantize_device", "b200idx_mx4_product_device",
     "b200idx_version",
 ]
 
@@ -452,3 +462,55 @@ def merge_topk_device(nsrc: int, n: int, k: int, descending: bool, Din_ptr: int,
                                            C.c_void_p(D_ptr), C.c_void_p(I_ptr), C.c_void_p(stream_ptr))
     if rc:
         raise B200IdxError(rc, "merge_topk_device failed")
+
+
+# ---- operators on rows in few bits (see include/b200idx.h).  Addresses of device memory, e.g.
+# ``tensor.data_ptr()``; work is queued on the stream, nothing is allocated or waited for. ----
+def rms_norm_i8_device(n: int, d: int, dtype: int, x_ptr: int, weight_ptr: int, eps: float, q_ptr: int, *,
+                       scales_ptr: int = 0, static_scale_ptr: int = 0, residual_ptr: int = 0, sum_ptr: int = 0,
+                       ldx: int = 0, ldr: int = 0, lds: int = 0, ldq: int = 0, stream_ptr: int = 0):
+    """x (+ residual) -> RMS norm -> int8 rows with a scale per row or one given scale: the rows of an Int8Flat index."""
+    _check(load().b200idx_rms_norm_i8_device(n, d, dtype, x_ptr, ldx, residual_ptr, ldr, sum_ptr, lds, weight_ptr, eps,
+                                             static_scale_ptr, q_ptr, ldq, scales_ptr, stream_ptr))
+
+
+def i8_dequantize_device(n: int, d: int, q_ptr: int, dtype: int, out_ptr: int, *, scales_ptr: int = 0,
+                         static_scale_ptr: int = 0, ldq: int = 0, ldo: int = 0, stream_ptr: int = 0):
+    """The values that int8 rows with scales stand for."""
+    _check(load().b200idx_i8_dequantize_device(n, d, q_ptr, ldq, scales_ptr, static_scale_ptr, dtype, out_ptr, ldo,
+                                               stream_ptr))
+
+
+def mx4_row_bytes(d: int) -> int:
+    """Bytes of the codes of one microscaled 4-bit row."""
+    return _positive(load().b200idx_mx4_row_bytes(d))
+
+
+def mx4_scale_bytes(n: int, d: int) -> int:
+    """Bytes of the scales of n microscaled 4-bit rows."""
+    return _positive(load().b200idx_mx4_scale_bytes(n, d))
+
+
+def _positive(v: int) -> int:
+    if v < 0:
+        raise B200IdxError(2001, "n must be > 0 and < 1e9, d in (0, 16384]")
+    return int(v)
+
+
+def mx4_quantize_device(n: int, d: int, dtype: int, x_ptr: int, codes_ptr: int, scales_ptr: int, *, ldx: int = 0,
+                        stream_ptr: int = 0):
+    """Rows -> microscaled 4-bit floating point (blocks of 32, E2M1 codes, E8M0 scales)."""
+    _check(load().b200idx_mx4_quantize_device(n, d, dtype, x_ptr, ldx, codes_ptr, scales_ptr, stream_ptr))
+
+
+def mx4_dequantize_device(n: int, d: int, codes_ptr: int, scales_ptr: int, dtype: int, out_ptr: int, *, ldo: int = 0,
+                          stream_ptr: int = 0):
+    """The values that microscaled 4-bit rows stand for."""
+    _check(load().b200idx_mx4_dequantize_device(n, d, codes_ptr, scales_ptr, dtype, out_ptr, ldo, stream_ptr))
+
+
+def mx4_product_device(m: int, n: int, d: int, a_codes_ptr: int, a_scales_ptr: int, b_codes_ptr: int,
+                       b_scales_ptr: int, dtype: int, out_ptr: int, *, ldo: int = 0, stream_ptr: int = 0):
+    """out[i][j] = sum_k a[i][k] b[j][k] of microscaled 4-bit rows, added up in fp32."""
+    _check(load().b200idx_mx4_product_device(m, n, d, a_codes_ptr, a_scales_ptr, b_codes_ptr, b_scales_ptr, dtype,
+                                             out_ptr, ldo, stream_ptr))

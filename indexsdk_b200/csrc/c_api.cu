@@ -137,6 +137,7 @@ bool descending_of(const b200idx_index* h) {
 
 namespace b200_capi {
 int guarded(const b200idx_t* h, const std::function<void()>& f) { return ::guarded(h, f); }
+int guarded_call(const std::function<void()>& f) { return guarded_create(f); }
 b200::FlatIndex* flat_of(b200idx_t* h) { return (h && h->kind != 2) ? h->flat.get() : nullptr; }
 }  // namespace b200_capi
 

@@ -1,0 +1,361 @@
+"""Operators on rows in few bits against plain 64-bit statements (tests/row_reference.py)."""
+import numpy as np
+import pytest
+import torch
+
+import row_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(rng, n, d, dtype, wide=0.5):
+    x = rng.standard_normal((n, d)) * np.exp(wide * rng.standard_normal(d))
+    return torch.from_numpy(x).to("cuda", ref.TORCH[dtype])
+
+
+def _strided(t, ld, offset=0):
+    """A copy of t with row stride ld, starting `offset` elements into its memory."""
+    n, d = t.shape
+    big = torch.zeros(n * ld + offset + 8, dtype=t.dtype, device="cuda")
+    v = big[offset:offset + n * ld].view(n, ld)[:, :d]
+    v.copy_(t)
+    return v
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ---- MX4 rounding ----
+def quantize(b, x, canary=True):
+    n, d = x.shape
+    pitch, sb = b.mx4_row_bytes(d), b.mx4_scale_bytes(n, d)
+    codes = torch.full((n * pitch + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    scales = torch.full((sb + 64,), 0xCD, dtype=torch.uint8, device="cuda")
+    dt = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[x.dtype]
+    b.mx4_quantize_device(n, d, dt, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), ldx=x.stride(0) if n > 1 else 0,
+                          stream_ptr=_stream())
+    assert bool((codes[n * pitch:] == 0xAB).all()) and bool((scales[sb:] == 0xCD).all())
+    return codes[:n * pitch].view(n, pitch), scales[:sb]
+
+
+def check_quantize(b, x):
+    n, d = x.shape
+    codes, scales = quantize(b, x)
+    rc, rs = ref.mx4_encode(x.double().cpu().numpy())
+    pc, ps = ref.mx4_pack(rc, rs, fill=0xCD)   # scale bytes of rows behind n stay as they were
+    np.testing.assert_array_equal(codes.cpu().numpy(), pc)
+    np.testing.assert_array_equal(scales.cpu().numpy(), ps)
+    return codes, scales, rc, rs
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n, d", [(1, 1), (1, 32), (3, 31), (5, 33), (2, 127), (130, 128), (129, 129), (7, 256), (33, 777),
+                                  (1, 4096), (300, 96), (2, 16384), (1, 16383), (1000, 8)])
+def test_mx4_quantize(b200, n, d, dtype):
+    rng = np.random.default_rng(n * 1000 + d)
+    check_quantize(b200, _rows(rng, n, d, dtype))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("ld, offset", [(100, 0), (104, 0), (101, 3), (128, 1)])
+def test_mx4_quantize_strides(b200, ld, offset, dtype):
+    x = _rows(np.random.default_rng(5), 37, 100, dtype)
+    check_quantize(b200, _strided(x, ld, offset))
+
+
+def test_mx4_quantize_borders_and_special_values(b200):
+    # every border between two codes, its neighbours in fp32, and both signs, at several scales
+    mids = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9999995], np.float32)
+    near = np.concatenate([mids, np.nextafter(mids, np.float32(0)), np.nextafter(mids, np.float32(8))])
+    near = np.minimum(near, np.float32(7.9999995))
+    rows = []
+    for e in (-126, -30, 0, 17, 125):
+        for lo in range(0, len(near), 15):
+            v = np.zeros(32, np.float32)
+            v[0] = 4.0   # keeps the block's scale at 2^0 before shifting
+            part = near[lo:lo + 15]
+            v[1:1 + len(part)] = part
+            v[16:16 + len(part)] = -part
+            rows.append((v.astype(np.float64) * 2.0 ** e).astype(np.float32))
+    tiny = np.float32(1e-45)
+    big = np.finfo(np.float32).max
+    for v in ([0.0], [-0.0, 0.0], [tiny], [2.0 ** -127, -tiny], [big, -big, 1.0], [np.nan, 1.0], [np.inf, 2.0], [-np.inf],
+              [2.0 ** -126, 2.0 ** -128]):
+        r = np.zeros(32, np.float32)
+        r[:len(v)] = v
+        rows.append(r)
+    x = torch.from_numpy(np.stack(rows)).cuda()
+    codes, scales, rc, rs = check_quantize(b200, x)
+    out = torch.empty(x.shape, device="cuda")
+    b200.mx4_dequantize_device(x.shape[0], 32, codes.data_ptr(), scales.data_ptr(), b200.F32, out.data_ptr())
+    np.testing.assert_array_equal(out.cpu().numpy(), ref.mx4_values(rc, rs, 32).astype(np.float32))
+    # a block that is not a number leaves its neighbours alone
+    y = torch.ones(2, 96, device="cuda")
+    y[1, 40] = float("nan")
+    check_quantize(b200, y)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n, d, ld", [(1, 1, 0), (3, 33, 0), (130, 128, 0), (7, 777, 780), (5, 100, 101), (2, 4096, 0)])
+def test_mx4_dequantize(b200, n, d, ld, dtype):
+    rng = np.random.default_rng(d)
+    rc, rs = ref.random_mx4(rng, n, d, spread=9)
+    pc, ps = ref.mx4_pack(rc, rs)
+    codes, scales = torch.from_numpy(pc).cuda(), torch.from_numpy(ps).cuda()
+    ld = ld or d
+    out = torch.full((n, ld), -7.0, dtype=ref.TORCH[dtype], device="cuda")
+    b200.mx4_dequantize_device(n, d, codes.data_ptr(), scales.data_ptr(), dtype, out.data_ptr(), ldo=ld, stream_ptr=_stream())
+    want = torch.from_numpy(ref.mx4_values(rc, rs, d)).to(ref.TORCH[dtype])   # one rounding, none for fp32 and bf16
+    assert torch.equal(out[:, :d].cpu(), want) and bool((out[:, d:] == -7.0).all())
+
+
+# ---- RMS norm -> int8 ----
+def rms(b, x, w, eps=1e-6, residual=None, static=None, in_place=None, ldq=0):
+    n, d = x.shape
+    dt = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[x.dtype]
+    ld = lambda t: t.stride(0) if n > 1 else 0  # noqa: E731
+    q = torch.full((n * (ldq or d) + 64,), 99, dtype=torch.int8, device="cuda")
+    scales = None if static is not None else torch.full((n + 4,), -5.0, device="cuda")
+    total = None
+    if residual is not None:
+        total = {"x": x, "residual": residual, None: torch.empty(n, d, dtype=x.dtype, device="cuda")}[in_place]
+    b.rms_norm_i8_device(n, d, dt, x.data_ptr(), w.data_ptr(), eps, q.data_ptr(), ldx=ld(x), ldq=ldq,
+                         residual_ptr=0 if residual is None else residual.data_ptr(),
+                         ldr=0 if residual is None else ld(residual),
+                         sum_ptr=0 if total is None else total.data_ptr(), lds=0 if total is None else ld(total),
+                         scales_ptr=0 if scales is None else scales.data_ptr(),
+                         static_scale_ptr=0 if static is None else static.data_ptr(), stream_ptr=_stream())
+    torch.cuda.synchronize()
+    assert bool((q[n * (ldq or d):] == 99).all()) and (scales is None or bool((scales[n:] == -5.0).all()))
+    rows = q[:n * (ldq or d)].view(n, ldq or d)
+    assert bool((rows[:, d:] == 99).all())
+    return rows[:, :d], None if scales is None else scales[:n], total
+
+
+def check_rms(x, w, eps, q, scales, total, residual=None, static=None):
+    s = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    if total is not None:
+        assert torch.equal(total, s)
+    y = ref.rms_norm(s.double().cpu().numpy(), w.double().cpu().numpy(), eps)
+    if static is None:
+        want = np.abs(y).max(1) / 127
+        # fp32: d squares added up in any order (d eps), root, quotient, products: under (d / 2 + 8) roundings,
+        # half of the sum's error left by the root; blockwise sums keep it far below that
+        tol = (s.shape[1] / 64 + 8) * ref.EPS[0]
+        np.testing.assert_allclose(scales.double().cpu().numpy(), want, rtol=tol, atol=0)
+        step = np.where(want > 0, want, 1.0)[:, None]
+    else:
+        step = float(static)
+    exact = np.clip(y / step, -127, 127)
+    # half a step, and the fp32 roundings of a value of at most 127 steps
+    off = np.abs(q.double().cpu().numpy() - exact)
+    assert off.max() <= 0.5 + 127 * (s.shape[1] / 64 + 8) * ref.EPS[0], off.max()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("n, d", [(1, 1), (1, 768), (5, 31), (3, 256), (9, 257), (4, 512), (2, 1000), (6, 1024), (3, 2048),
+                                  (2, 3001), (3, 4096), (2, 5000), (1, 8192), (2, 16384), (1, 16001)])
+def test_rms_norm_i8(b200, n, d, static, residual, dtype):
+    rng = np.random.default_rng(d + n)
+    x, w = _rows(rng, n, d, dtype), _rows(rng, 1, d, dtype, 0.0).view(-1)
+    r = _rows(rng, n, d, dtype) if residual else None
+    s = torch.tensor([0.021], device="cuda") if static else None
+    q, scales, total = rms(b200, x, w, residual=r, static=s)
+    check_rms(x, w, 1e-6, q, scales, total, r, s)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("ld, offset, ldq", [(104, 0, 104), (101, 3, 0), (112, 1, 103)])
+def test_rms_norm_strides(b200, ld, offset, ldq, dtype):
+    rng = np.random.default_rng(3)
+    x, r = (_strided(_rows(rng, 11, 100, dtype), ld, offset) for _ in range(2))
+    w = _rows(rng, 1, 100, dtype).view(-1)
+    q, scales, total = rms(b200, x, w, residual=r, ldq=ldq)
+    check_rms(x, w, 1e-6, q, scales, total, r)
+
+
+@pytest.mark.parametrize("place", ["x", "residual"])
+@pytest.mark.parametrize("d", [64, 77, 4096])
+def test_rms_norm_sum_in_place(b200, place, d):
+    rng = np.random.default_rng(4)
+    x, r, w = _rows(rng, 5, d, 2), _rows(rng, 5, d, 2), _rows(rng, 1, d, 2).view(-1)
+    x0, r0 = x.clone(), r.clone()
+    q, scales, total = rms(b200, x, w, residual=r, in_place=place)
+    check_rms(x0, w, 1e-6, q, scales, total, r0)
+    assert torch.equal(r if place == "x" else x, r0 if place == "x" else x0)
+
+
+def test_rms_norm_range(b200):
+    """Rows whose squares leave fp32, tiny rows, rows of zeros, rows that hold no numbers."""
+    d = 300
+    rng = np.random.default_rng(9)
+    base = rng.standard_normal((6, d)).astype(np.float32)
+    x = np.stack([base[0] * 1e30, base[1] * 1e-30, np.zeros(d, np.float32), base[3], base[4], base[5] * 3e37])
+    x[3, 7] = np.nan
+    x[4, 290] = np.inf
+    x = torch.from_numpy(x).cuda()
+    w = torch.from_numpy((1 + 0.1 * rng.standard_normal(d)).astype(np.float32)).cuda()
+    for residual in (None, torch.zeros_like(x)):
+        q, scales, total = rms(b200, x, w, residual=residual, in_place=None if residual is None else "x")
+        good = [0, 1, 5]
+        check_rms(x[good], w, 1e-6, q[good], scales[good], None)
+        assert float(scales[2]) == 0.0 and bool((q[2] == 0).all())
+        assert bool(torch.isnan(scales[3:5]).all()) and bool((q[3:5] == 0).all())
+    for s in (0.0, -1.0, float("nan"), float("inf")):
+        q, _, _ = rms(b200, x, w, static=torch.tensor([s], device="cuda"))
+        assert bool((q == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n, d, ldq, ldo", [(1, 1, 0, 0), (3, 100, 104, 101), (65, 96, 0, 0), (7, 4096, 0, 0)])
+def test_i8_dequantize(b200, n, d, ldq, ldo, dtype):
+    rng = np.random.default_rng(1)
+    q = torch.from_numpy(rng.integers(-128, 128, (n, ldq or d)).astype(np.int8)).cuda()
+    scales = torch.from_numpy(rng.random(n).astype(np.float32)).cuda()
+    out = torch.full((n, ldo or d), 3.0, dtype=ref.TORCH[dtype], device="cuda")
+    b200.i8_dequantize_device(n, d, q.data_ptr(), dtype, out.data_ptr(), scales_ptr=scales.data_ptr(), ldq=ldq, ldo=ldo,
+                              stream_ptr=_stream())
+    want = (q[:, :d].float() * scales[:, None]).to(ref.TORCH[dtype])
+    assert torch.equal(out[:, :d], want) and bool((out[:, d:] == 3.0).all())
+    b200.i8_dequantize_device(n, d, q.data_ptr(), dtype, out.data_ptr(), static_scale_ptr=scales.data_ptr(), ldq=ldq,
+                              ldo=ldo, stream_ptr=_stream())
+    assert torch.equal(out[:, :d], (q[:, :d].float() * scales[0]).to(ref.TORCH[dtype]))
+
+
+# ---- MX4 product ----
+def product(b, m, n, d, a, bb, dtype=0, ldo=0):
+    out = torch.full((m * (ldo or n) + 16,), -3.0, dtype=ref.TORCH[dtype], device="cuda")
+    b.mx4_product_device(m, n, d, a[0].data_ptr(), a[1].data_ptr(), bb[0].data_ptr(), bb[1].data_ptr(), dtype, out.data_ptr(),
+                         ldo=ldo, stream_ptr=_stream())
+    torch.cuda.synchronize()
+    assert bool((out[m * (ldo or n):] == -3.0).all())
+    rows = out[:m * (ldo or n)].view(m, ldo or n)
+    assert bool((rows[:, n:] == -3.0).all())
+    return rows[:, :n]
+
+
+def random_operand(rng, n, d, spread=2, fill=127):
+    c, s = ref.random_mx4(rng, n, d, spread)
+    p, t = ref.mx4_pack(c, s, fill)
+    return (torch.from_numpy(p).cuda(), torch.from_numpy(t).cuda()), ref.mx4_values(c, s, d)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("m, n, d", [(1, 1, 1), (1, 64, 32), (2, 300, 64), (3, 257, 33), (17, 1000, 128), (64, 129, 160),
+                                     (65, 511, 256), (127, 256, 288), (128, 257, 1000), (129, 300, 96), (200, 70, 544),
+                                     (1, 5000, 768), (16, 4096, 2048), (5, 130, 4096), (300, 600, 4100), (2, 40, 16384)])
+def test_mx4_product(b200, m, n, d, dtype):
+    """Sums that fp32 holds exactly: products are quarters times at least 2^-4, sums stay below 2^24 of those
+    (|sum| <= 36 d 2^2, in steps of 2^-6: d <= 2^24 / (36 * 2^8) = 1820; longer rows use equal scales:
+    d <= 2^24 / (36 * 4)).  Equality, then, or one rounding to 16 bits."""
+    rng = np.random.default_rng(m * 7 + n + d)
+    spread = 1 if d <= 1800 else 0
+    # rows behind m and n have scale bytes that stand for NaN: nobody may see them
+    if spread:
+        a, va = random_operand(rng, m, d, spread, fill=255)
+        bb, vb = random_operand(rng, n, d, spread, fill=255)
+    else:
+        ca, cb = ref.random_mx4(rng, m, d)[0], ref.random_mx4(rng, n, d)[0]
+        nb = -(-d // 32)
+        sa, sb = np.full((m, nb), 126, np.uint8), np.full((n, nb), 129, np.uint8)
+        a = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(ca, sa, 255)]
+        bb = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(cb, sb, 255)]
+        va, vb = ref.mx4_values(ca, sa, d), ref.mx4_values(cb, sb, d)
+    want = torch.from_numpy(va @ vb.T).to(ref.TORCH[dtype]).cuda()
+    assert torch.equal(product(b200, m, n, d, a, bb, dtype), want)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("ldo", [301, 304, 512])
+def test_mx4_product_output_stride(b200, ldo, dtype):
+    rng = np.random.default_rng(2)
+    for m in (3, 140):
+        a, va = random_operand(rng, m, 96)
+        bb, vb = random_operand(rng, 300, 96)
+        want = torch.from_numpy(va @ vb.T).to(ref.TORCH[dtype]).cuda()
+        assert torch.equal(product(b200, m, 300, 96, a, bb, dtype, ldo), want)
+
+
+@pytest.mark.parametrize("m", [1, 7, 33, 150])
+def test_mx4_product_wide_scales(b200, m):
+    """Scales across the whole range of the format; sums round."""
+    rng = np.random.default_rng(8)
+    n, d = 200, 512
+    ca, cb = ref.random_mx4(rng, m, d)[0], ref.random_mx4(rng, n, d)[0]
+    sa = rng.integers(87, 168, (m, d // 32)).astype(np.uint8)
+    sb = rng.integers(87, 168, (n, d // 32)).astype(np.uint8)
+    a = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(ca, sa)]
+    bb = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(cb, sb)]
+    va, vb = ref.mx4_values(ca, sa, d), ref.mx4_values(cb, sb, d)
+    got = product(b200, m, n, d, a, bb).double().cpu().numpy()
+    # d additions of terms of that size, each off by at most a step (the tensor core may cut instead of round)
+    tol = 2 * ref.EPS[0] * d * (np.abs(va) @ np.abs(vb).T)
+    assert np.all(np.abs(got - va @ vb.T) <= tol)
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_mx4_product_nan_blocks(b200, m):
+    """A block that stands for NaN makes its row's scores NaN and nobody else's."""
+    rng = np.random.default_rng(6)
+    n, d = 150, 100
+    ca, sa = ref.random_mx4(rng, m, d)
+    cb, sb = ref.random_mx4(rng, n, d)
+    sa[0, 1], ca[0, 32:64] = 255, 0
+    sb[149, 3], cb[149, 96:128] = 255, 0
+    a = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(ca, sa)]
+    bb = [torch.from_numpy(t).cuda() for t in ref.mx4_pack(cb, sb)]
+    got = product(b200, m, n, d, a, bb).cpu().numpy()
+    bad = np.zeros((m, n), bool)
+    bad[0], bad[:, 149] = True, True
+    want = ref.mx4_values(ca, sa, d) @ ref.mx4_values(cb, sb, d).T
+    np.testing.assert_array_equal(np.isnan(got), bad)
+    np.testing.assert_array_equal(got[~bad], want[~bad].astype(np.float32))
+
+
+# ---- the operators as they are used ----
+def test_states_to_scores(b200):
+    """fp16 states -> RMS norm -> int8 -> values -> MX4 -> scores, one after the other on a stream of their own,
+    while that stream is not the current one's default; then the same captured and replayed on new states."""
+    rng = np.random.default_rng(11)
+    n, m, d = 70, 9, 200
+    st = torch.cuda.Stream()
+    x = _rows(rng, n, d, 1)
+    w = _rows(rng, 1, d, 1, 0.1).view(-1)
+    q = torch.empty(n, d, dtype=torch.int8, device="cuda")
+    sc = torch.empty(n, device="cuda")
+    val = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    codes = torch.empty(n, b200.mx4_row_bytes(d), dtype=torch.uint8, device="cuda")
+    scales = torch.empty(b200.mx4_scale_bytes(n, d), dtype=torch.uint8, device="cuda")
+    out = torch.empty(m, n, device="cuda")
+
+    def chain(s):
+        b200.rms_norm_i8_device(n, d, b200.F16, x.data_ptr(), w.data_ptr(), 1e-6, q.data_ptr(), scales_ptr=sc.data_ptr(),
+                                stream_ptr=s)
+        b200.i8_dequantize_device(n, d, q.data_ptr(), b200.BF16, val.data_ptr(), scales_ptr=sc.data_ptr(), stream_ptr=s)
+        b200.mx4_quantize_device(n, d, b200.BF16, val.data_ptr(), codes.data_ptr(), scales.data_ptr(), stream_ptr=s)
+        b200.mx4_product_device(m, n, d, codes.data_ptr(), scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), b200.F32,
+                                out.data_ptr(), stream_ptr=s)
+
+    def check():
+        check_rms(x, w, 1e-6, q, sc, None)
+        assert torch.equal(val, (q.float() * sc[:, None]).bfloat16())
+        rc, rs = ref.mx4_encode(val.double().cpu().numpy())
+        v = ref.mx4_values(rc, rs, d)
+        np.testing.assert_allclose(out.double().cpu().numpy(), (v @ v.T)[:m], rtol=0,
+                                   atol=2 * ref.EPS[0] * d * float((np.abs(v) @ np.abs(v).T).max()))
+
+    torch.cuda.synchronize()
+    chain(st.cuda_stream)
+    torch.cuda.synchronize()
+    check()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chain(_stream())
+    for seed in (12, 13):
+        x.copy_(_rows(np.random.default_rng(seed), n, d, 1))
+        g.replay()
+        torch.cuda.synchronize()
+        check()
