@@ -132,4 +132,8 @@ cudaError_t launch_dist_gemm(const GemmLaunch& L, const GemmArgs& a, const CUten
 // Returns 0 on success.
 int encode_operand_map(CUtensorMap* out, int kind, const void* base, int64_t rows, int d, int box_rows);
 
+// The same for any row-major array: rows of `cols` elements of elem_bytes each.
+int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem_bytes, const void* base, int64_t rows, int cols,
+                    int box_rows);
+
 }  // namespace b200

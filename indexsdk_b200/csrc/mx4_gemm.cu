@@ -1,60 +1,356 @@
+// Products of microscaled 4-bit rows with tcgen05.mma kind::mxf4 (E2M1 codes, a scale per 32 elements).
+//
+// A CTA computes 128 x 256 tiles (rows of a x rows of b) of fp32 accumulators in TMEM:
+//   warp 0 (one lane)  : producer.  Per K chunk of 128 bytes (256 elements) two tensor copies (128 and 256 rows,
+//                        SWIZZLE_128B) and up to three copies of scales into a ring of four 51 KB stages.  The
+//                        scales lie in memory in the order the tensor core wants, 512 bytes for 128 rows x 4
+//                        blocks, so nothing is rearranged on the way.
+//   warp 1 (one lane)  : copies a stage's scales into TMEM (tcgen05.cp, a slot of 24 columns per stage) and issues
+//                        up to four 128 x 256 x 64 products.
+//   warps 2-17         : epilogue.  Thread = (row, 64 of the tile's 256 columns), both 32-column chunks in
+//                        registers at once, so that the accumulator goes back before the slow part begins.
+// TMEM has 512 columns: two accumulators of 256 and the 96 columns of scales do not fit side by side.  The two
+// accumulators therefore SHARE 96 columns (0-255 and 160-415; scales 416-511): tile t + 1 may start once tile t's
+// shared columns are in registers, which half of the epilogue warps report.
 #include "mx4_gemm.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
+#include "ptx_sm100.cuh"
+#include "row_epilogue.cuh"
 #include "row_ops.cuh"
+#include "smem_limit.h"
 
 namespace b200 {
 namespace {
 
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-    return byte == 0u ? __int_as_float(0x00400000) : __int_as_float(byte == 255u ? 0x7fc00000 : byte << 23);
-}
-// twice the value of a code
-__device__ __forceinline__ int code2(uint32_t c) {
-    const int m = static_cast<int>(0xC8643210u >> (4 * (c & 7u)) & 15u);
-    return c & 8u ? -m : m;
+constexpr int kStages = 4;
+constexpr int kABytes = kTileQ * kChunkBytes, kBBytes = kTileB * kChunkBytes;   // 16 KB, 32 KB
+constexpr int kSfaBytes = 1024, kSfbBytes = 2048;                               // two groups of 128 elements
+constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;          // 51 KB
+constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kEpiWarps = 16;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kAcc1 = 160, kScaleCols = 416, kScaleSlot = 24;   // TMEM columns
+constexpr int kModeDense = 2;
+
+struct Mx4Args {
+    GemmArgs g;
+    const uint8_t* a_scales;
+    const uint8_t* b_scales;
+    int nb, ng;      // blocks of a row, groups of four
+    // kModeDense
+    void* out;
+    int64_t ldo;
+    int dtype;
+    int vec;         // rows of out start on 16-byte boundaries
+};
+
+// 32 accumulator columns of one row -> out[0 .. nvalid)
+template <typename T>
+__device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], T* o, int nvalid, bool vec) {
+    constexpr int kPer = 16 / sizeof(T);
+    if (vec && nvalid >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32 / kPer; ++i) {
+            uint4 u;
+            if constexpr (sizeof(T) == 4) {
+                u = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float lo = __uint_as_float(r[8 * i + 2 * j]), hi = __uint_as_float(r[8 * i + 2 * j + 1]);
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const __half2 h = __floats2half2_rn(lo, hi);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+                u = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            reinterpret_cast<uint4*>(o)[i] = u;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            if (c < nvalid) {
+                const float v = __uint_as_float(r[c]);
+                if constexpr (std::is_same<T, float>::value) o[c] = v;
+                else if constexpr (std::is_same<T, __half>::value) o[c] = __float2half_rn(v);
+                else o[c] = __float2bfloat16_rn(v);
+            }
+        }
+    }
 }
 
-// A thread per output: the 32 products of a block are whole quarters, so their sum is exact.
-template <typename T>
-__global__ void __launch_bounds__(256) mx4_product_kernel(const Mx4ProductArgs a) {
-    const int nb = mx4_blocks(a.d), ng = mx4_groups(a.d);
-    const int64_t pitch = mx4_pitch(a.d), total = a.m * a.n;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / a.n, c = i - r * a.n;
-        const uint4* pa = reinterpret_cast<const uint4*>(a.a_codes + r * pitch);
-        const uint4* pb = reinterpret_cast<const uint4*>(a.b_codes + c * pitch);
-        float acc = 0.f;
-        for (int b = 0; b < nb; ++b) {
-            const uint4 va = pa[b], vb = pb[b];
-            const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-            int dot = 0;
-            for (int w = 0; w < 4; ++w)
-                for (int e = 0; e < 8; ++e) dot += code2(wa[w] >> (4 * e) & 15u) * code2(wb[w] >> (4 * e) & 15u);
-            const float sa = scale_value(a.a_scales[mx4_scale_word(r, b >> 2, ng) + (b & 3)]);
-            const float sb = scale_value(a.b_scales[mx4_scale_word(c, b >> 2, ng) + (b & 3)]);
-            acc += 0.25f * static_cast<float>(dot) * sa * sb;
+template <int MODE, int BURST, bool L2>
+__global__ void __launch_bounds__(kThreads, 1)
+mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Mx4Args m) {
+    const GemmArgs& a = m.g;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[kStages], bar_empty[kStages], bar_acc_full[2], bar_shared_free;
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int nkc = (m.ng + 1) / 2;   // chunks of 256 elements
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(&bar_full[s], 1);
+            ptx::mbar_init(&bar_empty[s], 1);
         }
-        T* o = static_cast<T*>(a.out) + r * a.ldo + c;
-        if constexpr (std::is_same<T, float>::value) *o = acc;
-        else if constexpr (std::is_same<T, __half>::value) *o = __float2half_rn(acc);
-        else *o = __float2bfloat16_rn(acc);
+        ptx::mbar_init(&bar_acc_full[0], 1);
+        ptx::mbar_init(&bar_acc_full[1], 1);
+        ptx::mbar_init(&bar_shared_free, kEpiWarps / 2);
+        abort_flag = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&mapA);
+        ptx::prefetch_tensormap(&mapB);
     }
+    if (warp == 1) {
+        ptx::tmem_alloc(&tmem_base_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+    const int n_qb = (a.nq + kTileQ - 1) / kTileQ;
+    const ItemRange range(a, n_qb);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            ItemCursor cur(range);
+            const int64_t b_granules = (a.N + 127) / 128;
+            for (int64_t i = 0; i < range.count && ok; ++i, cur.next()) {
+                const int64_t tile = tile_of(a, cur.sel);
+                const bool second = 2 * tile + 1 < b_granules;   // the tile's upper 128 rows exist
+                const uint8_t* sa = m.a_scales + static_cast<int64_t>(cur.qb) * m.ng * 512;
+                const uint8_t* sb = m.b_scales + 2 * tile * m.ng * 512;
+                for (int kc = 0; kc < nkc; ++kc) {
+                    if (!ptx::mbar_wait_bounded(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                    uint8_t* st = smem + s * kStageBytes;
+                    const uint32_t sf = min(2, m.ng - 2 * kc) * 512u;
+                    ptx::mbar_expect_tx(&bar_full[s], kABytes + kBBytes + sf * (second ? 3u : 2u));
+                    ptx::tma_load_2d(st, &mapA, &bar_full[s], kc * kChunkBytes, cur.qb * kTileQ);
+                    ptx::tma_load_2d(st + kABytes, &mapB, &bar_full[s], kc * kChunkBytes, static_cast<int>(tile * kTileB));
+                    ptx::bulk_load_1d(st + kABytes + kBBytes, sa + kc * 1024, sf, &bar_full[s]);
+                    ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes, sb + kc * 1024, sf, &bar_full[s]);
+                    if (second)
+                        ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes + 1024, sb + m.ng * 512 + kc * 1024, sf, &bar_full[s]);
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 0), kIdesc2 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 2);
+            const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
+            const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
+            const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
+            uint32_t s = 0, ph = 0, t = 0;
+            bool ok = true;
+            for (int64_t i = 0; i < range.count && ok; ++i, ++t) {
+                // the columns this accumulator shares with tile t - 1's (and with them all of tile t - 2's)
+                if (t && !ptx::mbar_wait_bounded(&bar_shared_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + (t & 1u ? kAcc1 : 0u);
+                for (int kc = 0; kc < nkc; ++kc) {
+                    if (!ptx::mbar_wait_bounded(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+                    const uint32_t st = ring_lo + s * (kStageBytes >> 4);
+                    const uint32_t sf_lo = st + ((kABytes + kBBytes) >> 4);
+                    const uint32_t slot = tmem_base + kScaleCols + s * kScaleSlot;
+                    const int groups = min(2, m.ng - 2 * kc);
+                    for (int g = 0; g < groups; ++g) {   // slot: 4 columns of a's scales, 8 of b's, per group
+                        const uint32_t col = slot + g * 12;
+                        ptx::tmem_cp_scales(col, sf_hi | static_cast<uint64_t>(sf_lo + g * 32));
+                        ptx::tmem_cp_scales(col + 4, sf_hi | static_cast<uint64_t>(sf_lo + 64 + g * 32));
+                        ptx::tmem_cp_scales(col + 8, sf_hi | static_cast<uint64_t>(sf_lo + 128 + g * 32));
+                    }
+                    const int steps = min(4, (m.nb - 8 * kc + 1) / 2);   // 64 elements each
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks >= steps) break;
+                        const uint32_t col = slot + (ks >> 1) * 12;
+                        ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                       desc_hi | static_cast<uint64_t>(st + (kABytes >> 4) + ks * 2),
+                                       (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
+                    }
+                    ptx::umma_commit(&bar_empty[s]);
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                ptx::umma_commit(&bar_acc_full[t & 1u]);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, part = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
+        const uint32_t* gnorm = static_cast<const uint32_t*>(a.bnorm);
+        RowEpilogue<float, MODE == kModeDense ? kModeAppend : MODE, BURST, false, 2, false, !L2> epi(a);
+        uint32_t t = 0;
+        bool ok = true;
+        ItemCursor cur(range);
+        for (int64_t i = 0; i < range.count; ++i, ++t, cur.next()) {
+            const int sel = cur.sel, q = cur.qb * kTileQ + quarter * 32 + lane;
+            const int64_t tile = tile_of(a, sel);
+            const int64_t col0 = tile * kTileB + part * 64;
+            const uint32_t ab = t & 1u;
+            const int64_t rem = a.N - col0;
+            const int va = rem >= 32 ? 32 : (rem > 0 ? static_cast<int>(rem) : 0);
+            const int vb = rem >= 64 ? 32 : (rem > 32 ? static_cast<int>(rem) - 32 : 0);
+            uint32_t ra[32], rb[32];
+            if (MODE != kModeDense) epi.begin_tile(q, q < a.nq);
+            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
+            if (ok) {
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + (ab ? kAcc1 : 0u) + part * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
+                ptx::tmem_ld_32x32(tacc, ra);
+                ptx::tmem_ld_32x32(tacc + 32, rb);
+                ptx::tmem_ld_wait(ra);
+                ptx::tmem_ld_wait(rb);
+                ptx::tc_fence_before();
+                __syncwarp();
+                // shared columns: 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
+                if (lane == 0 && (ab ? part < 2 : part >= 2)) ptx::mbar_arrive(&bar_shared_free);
+            } else if (MODE != kModeDense) {
+                break;   // the host sees the error word
+            } else {
+                // nobody reads an error word behind a product: results that could not be computed are no numbers
+#pragma unroll
+                for (int c = 0; c < 32; ++c) ra[c] = rb[c] = 0x7fffffffu;
+            }
+            if (MODE == kModeDense) {
+                if (q < a.nq && va > 0) {
+                    const int64_t at = static_cast<int64_t>(q) * m.ldo + col0;
+                    const bool vec = m.vec != 0;
+                    if (m.dtype == kF32) {
+                        store_chunk(ra, static_cast<float*>(m.out) + at, va, vec);
+                        store_chunk(rb, static_cast<float*>(m.out) + at + 32, vb, vec);
+                    } else if (m.dtype == kF16) {
+                        store_chunk(ra, static_cast<__half*>(m.out) + at, va, vec);
+                        store_chunk(rb, static_cast<__half*>(m.out) + at + 32, vb, vec);
+                    } else {
+                        store_chunk(ra, static_cast<__nv_bfloat16*>(m.out) + at, va, vec);
+                        store_chunk(rb, static_cast<__nv_bfloat16*>(m.out) + at + 32, vb, vec);
+                    }
+                }
+                continue;
+            }
+            if (MODE == kModeAppend && !a.direct) {
+                const uint32_t* gn = gnorm + col0;
+                if (L2) {
+                    epi.l2_extract(ra, epi.l2_mask(ra, gn, col0, va), col0, gn);
+                    epi.l2_extract(rb, epi.l2_mask(rb, gn + 32, col0 + 32, vb), col0 + 32, gn + 32);
+                } else {
+                    epi.ip_extract(ra, epi.ip_mask(ra, col0, va), col0);
+                    epi.ip_extract(rb, epi.ip_mask(rb, col0 + 32, vb), col0 + 32);
+                }
+                epi.end_tile(0);
+            } else {
+                const int slot = sel * (kTileB / BURST) + part * (64 / BURST);
+                epi.chunk(ra, gnorm + col0, col0, va, slot, 0, 0);
+                epi.chunk(rb, gnorm + col0 + 32, col0 + 32, vb, slot + 32 / BURST, 1, 0);
+                epi.end_tile(slot);
+            }
+        }
+        if (MODE != kModeDense) epi.finish();
+    }
+
+    // After an abort, copies in flight get time to land before the CTA's shared memory is released.
+    __syncwarp();
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) { }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, 512);
+    }
+    if (MODE != kModeDense && threadIdx.x == 0 && abort_flag) atomicOr(a.err, kDevErrPipelineTimeout);
+}
+
+template <int MODE, int BURST, bool L2>
+cudaError_t launch_one(Mx4Args m, const CUtensorMap* mapA, const CUtensorMap* mapB, int num_sms, cudaStream_t stream) {
+    GemmArgs& a = m.g;
+    const int n_qb = (a.nq + kTileQ - 1) / kTileQ;
+    const int64_t total = static_cast<int64_t>(n_qb) * a.n_tiles_sel;
+    if (total <= 0) return cudaSuccess;
+    if (a.tile_step < 1) a.tile_step = 1;
+    auto kern = mx4_gemm_kernel<MODE, BURST, L2>;
+    cudaError_t e = allow_max_smem(kern);
+    if (e != cudaSuccess) return e;
+    const int grid = static_cast<int>(std::min<int64_t>(total, num_sms));
+    // CTAs of different query blocks on the same stretch of the base at the same time, where the split stays even
+    a.aligned_ranges = 0;
+    if (n_qb <= grid && a.n_tiles_sel >= grid / n_qb) {
+        const int nl_min = grid / n_qb;
+        const double worst = static_cast<double>((a.n_tiles_sel + nl_min - 1) / nl_min);
+        if (worst <= 1.06 * (static_cast<double>(total) / grid) + 1.0) a.aligned_ranges = 1;
+    }
+    const bool shared = n_qb == 1 && a.row_cands < 3LL * 4 * grid;   // (the rule of launch_dist_gemm)
+    a.eager = total >= 16LL * grid && !shared ? 1 : 0;
+    kern<<<grid, kThreads, kSmemBytes, stream>>>(*mapA, *mapB, m);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-void launch_mx4_product(int dtype, const Mx4ProductArgs& a, cudaStream_t st) {
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.m * a.n + 255) / 256, 148 * 64));
-    if (dtype == kF32) mx4_product_kernel<float><<<blocks, 256, 0, st>>>(a);
-    else if (dtype == kF16) mx4_product_kernel<__half><<<blocks, 256, 0, st>>>(a);
-    else mx4_product_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a);
-    B200_CUDA_CHECK(cudaGetLastError());
+void launch_mx4_product(int dtype, const Mx4ProductArgs& p, int num_sms, cudaStream_t st) {
+    CUtensorMap map_a, map_b;
+    if (encode_mx4_map(&map_a, p.a_codes, p.m, p.d, kTileQ) != 0 || encode_mx4_map(&map_b, p.b_codes, p.n, p.d, kTileB) != 0)
+        throw std::runtime_error("cuTensorMapEncodeTiled failed for the rows of a product");
+    Mx4Args m{};
+    m.g.nq = static_cast<int>(p.m);
+    m.g.N = p.n;
+    m.g.d = p.d;
+    m.g.n_tiles_total = m.g.n_tiles_sel = div_up(p.n, kTileB);
+    m.a_scales = p.a_scales;
+    m.b_scales = p.b_scales;
+    m.nb = mx4_blocks(p.d);
+    m.ng = mx4_groups(p.d);
+    m.out = p.out;
+    m.ldo = p.ldo;
+    m.dtype = dtype;
+    const int size = dtype == kF32 ? 4 : 2;
+    m.vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * size % 16 == 0;
+    B200_CUDA_CHECK((launch_one<kModeDense, 32, false>(m, &map_a, &map_b, num_sms, st)));
+}
+
+cudaError_t launch_mx4_dist(const GemmLaunch& L, const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales,
+                            const CUtensorMap* mapA, const CUtensorMap* mapB, cudaStream_t stream) {
+    Mx4Args m{};
+    m.g = a;
+    m.a_scales = a_scales;
+    m.b_scales = b_scales;
+    m.nb = mx4_blocks(a.d);
+    m.ng = mx4_groups(a.d);
+    const bool l2 = a.metric == kMetricL2;
+    if (L.mode == kModeAppend)
+        return l2 ? launch_one<kModeAppend, 32, true>(m, mapA, mapB, L.num_sms, stream)
+                  : launch_one<kModeAppend, 32, false>(m, mapA, mapB, L.num_sms, stream);
+    if (L.burst == 8)
+        return l2 ? launch_one<kModeBurstMin, 8, true>(m, mapA, mapB, L.num_sms, stream)
+                  : launch_one<kModeBurstMin, 8, false>(m, mapA, mapB, L.num_sms, stream);
+    return l2 ? launch_one<kModeBurstMin, 32, true>(m, mapA, mapB, L.num_sms, stream)
+              : launch_one<kModeBurstMin, 32, false>(m, mapA, mapB, L.num_sms, stream);
+}
+
+int encode_mx4_map(CUtensorMap* out, const uint8_t* codes, int64_t rows, int d, int box_rows) {
+    return encode_rows_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, static_cast<int>(mx4_pitch(d)), box_rows);
 }
 
 }  // namespace b200

@@ -66,6 +66,12 @@ int device_of(std::initializer_list<Operand> ops) {
     return device;
 }
 
+int sm_count(int device) {
+    int sms = 0;
+    B200_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    return sms;
+}
+
 }  // namespace
 
 extern "C" {
@@ -143,10 +149,11 @@ int b200idx_mx4_product_device(int64_t m, int64_t n, int d, const uint8_t* a_cod
         check_dim(d);
         const size_t eb = elem_bytes(dtype);
         if (ldo != 0 && ldo < n) throw std::invalid_argument("ldo must be 0 or >= n");
-        DeviceGuard g(device_of({{"a_codes", a_codes, 16}, {"a_scales", a_scales, 16}, {"b_codes", b_codes, 16},
-                                 {"b_scales", b_scales, 16}, {"out", out, eb}}));
+        const int device = device_of({{"a_codes", a_codes, 16}, {"a_scales", a_scales, 16}, {"b_codes", b_codes, 16},
+                                      {"b_scales", b_scales, 16}, {"out", out, eb}});
+        DeviceGuard g(device);
         launch_mx4_product(dtype, Mx4ProductArgs{m, n, d, a_codes, a_scales, b_codes, b_scales, out, ldo ? ldo : n},
-                           static_cast<cudaStream_t>(stream));
+                           sm_count(device), static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -196,6 +196,30 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
         : "memory");
 }
 
+// Instruction descriptor of kind::mxf4 (E2M1 operands, E8M0 scales, fp32 accumulator, K = 64, both K-major).
+// The two scale bytes of a K step are bytes 0-1 or 2-3 of the 32-bit words at the scale addresses (sf_id 0 or 2).
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(uint32_t M, uint32_t N, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | (sf_id << 29);
+}
+// sfa, sfb: TMEM addresses of the scales.  Row r's word is at lane r % 32, column r / 32 (and in the same lane
+// of the other three quarters, where tcgen05.cp.warpx4 puts copies).
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// 512 bytes of shared memory (32 rows of 16 bytes, groups of 8 rows 128 bytes apart) -> 4 TMEM columns, the
+// same 32 lanes in every quarter.  Executes in order with the tcgen05.mma the same thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // Arrive on an mbarrier once all tcgen05.mma issued so far by this thread have completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
