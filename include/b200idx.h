@@ -48,6 +48,11 @@ enum {
  *   F16: fp16 rows, fp32 accumulation (the reference's own Flat arithmetic,
  *        FR/ascend/impl/AscendIndexImpl.cpp:339-346). */
 enum { B200IDX_F32 = 0, B200IDX_F16 = 1 };
+/*   MX4: float rows in, kept as microscaled 4-bit floating point (see below; 17 bytes for 32 elements), fp32
+ *        accumulation.  Queries are rounded the same way: distances and scores are those of the rounded
+ *        vectors, ties go to the lower position, a row or query with a block that stands for NaN has no
+ *        results.  b200idx_get_base gives the values that the rows stand for.  (No reference counterpart.) */
+enum { B200IDX_MX4 = 4 };
 /* Element type of rows in device memory that the operators below read or write, besides the two above. */
 enum { B200IDX_BF16 = 2 };
 
@@ -80,7 +85,7 @@ int b200idx_search_f16(b200idx_t* h, int64_t n, const uint16_t* x, int k, float*
  * i / 8 of a row is 1 when base position i (add order) may appear in that query's result (replaces
  * AscendIndexFlat::search_with_masks, feature_retrieval/src/ascendfaiss/ascend/AscendIndexFlat.h:78-82;
  * device predicate feature_retrieval/src/ascendfaiss/ops/ascendc/op_kernel/distance_flat_l2.cpp:487-533).
- * Flat and Int8Flat indexes; queries in the index's input dtype (float for F32 / F16 indexes). */
+ * Flat and Int8Flat indexes; queries in the index's input dtype (float for F32 / F16 / MX4 indexes). */
 int b200idx_search_with_masks(b200idx_t* h, int64_t n, const void* x, int k, const uint8_t* mask, float* distances,
                               int64_t* labels);
 
@@ -93,7 +98,7 @@ int b200idx_search_device(b200idx_t* h, int64_t n, const void* x_dev, int k, flo
  * operators always draw temporaries from a per-index pool).  For callers that may not allocate
  * device memory while searching -- a process whose HBM is owned by its own pool, or a loop that
  * cannot take the device-wide synchronisation of cudaMalloc / cudaFree.  Same kernels and same
- * results as b200idx_search_device on a Flat or Int8Flat index, with every scratch buffer taken
+ * results as b200idx_search_device on a Flat (not MX4) or Int8Flat index, with every scratch buffer taken
  * from one static device array of 9 MiB + 96 KiB: n * round_up(ntotal, 256) <= 2^20, k <= 1024,
  * n * k <= 131072, n * d <= 524288; anything larger returns B200IDX_ERR_INVALID_PARAM.  Calls
  * share that array: do not overlap two of them on one GPU.  The first call on a device resolves
@@ -145,8 +150,8 @@ int b200idx_merge_topk_device_strided(int nsrc, int64_t n, int k, int descending
  *
  * Root-mean-square norm with the residual's addition, rounded to int8 rows with scales: the last step of an
  * embedding model and what an Int8Flat index stores, in one pass.  Per row of x (type dtype: F32, F16, BF16)
- *   s = x + residual            rounded to dtype and written to `sum` (residual NULL: s = x, sum must be NULL;
- *                               sum may be x or residual itself, with the same stride)
+ *   s = x + residual            rounded to dtype and written to `sum` where that is given (residual NULL: s = x,
+ *                               sum must be NULL; sum may be x or residual itself, with the same stride)
  *   y = s / sqrt(mean(s^2) + eps) * weight          weight[d] in dtype, 1e-12 <= eps <= 1
  *   q = round(y / scale) to nearest, ties to even, cut to [-127, 127];  q has row stride ldq
  *   scale: static_scale[0] where that is given, else max|y| / 127 of the row, written to scales[n]
@@ -155,6 +160,16 @@ int b200idx_merge_topk_device_strided(int nsrc, int64_t n, int k, int descending
 int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64_t ldx, const void* residual,
                                int64_t ldr, void* sum, int64_t lds, const void* weight, float eps,
                                const float* static_scale, int8_t* q, int64_t ldq, float* scales, void* stream);
+/* The same as the way into an Int8Flat index (kind int8 only): the rows of n states on the index's device become
+ * vectors of the index, or queries.  States and residual are n x dim(h) without gaps, ready when the call is
+ * made; the calls return when they are done.  Rows of one index are comparable under INNER_PRODUCT and L2 when
+ * they share a scale, so these metrics take a static_scale, the same for base and queries; INT8_COSINE, which
+ * does not depend on it, also takes NULL (a scale per row). */
+int b200idx_add_states_device(b200idx_t* h, int64_t n, int dtype, const void* x, const void* residual, const void* weight,
+                              float eps, const float* static_scale, const int64_t* ids_host);
+int b200idx_search_states_device(b200idx_t* h, int64_t n, int dtype, const void* x, const void* residual,
+                                 const void* weight, float eps, const float* static_scale, int k, float* distances_dev,
+                                 int64_t* labels_dev);
 /* The values that int8 rows stand for, out = q * scale in dtype (exactly one of scales, static_scale is NULL). */
 int b200idx_i8_dequantize_device(int64_t n, int d, const int8_t* q, int64_t ldq, const float* scales,
                                  const float* static_scale, int dtype, void* out, int64_t ldo, void* stream);
@@ -192,7 +207,7 @@ int b200idx_remove_ids(b200idx_t* h, int64_t n, const int64_t* ids, int64_t* n_r
 int64_t b200idx_ntotal(const b200idx_t* h);
 int b200idx_dim(const b200idx_t* h);
 int b200idx_device(const b200idx_t* h);
-/* rows [offset, offset+n): float (F32), fp16 bits (F16) or int8 */
+/* rows [offset, offset+n): float (F32, MX4), fp16 bits (F16) or int8 */
 int b200idx_get_base(const b200idx_t* h, int64_t offset, int64_t n, void* out);
 int b200idx_get_ids(const b200idx_t* h, int64_t offset, int64_t n, int64_t* out);
 

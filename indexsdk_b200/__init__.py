@@ -21,6 +21,7 @@ METRIC_INT8_COSINE = 2     # Int8Flat only: the reference's fp16 cosine (see inc
 F32 = 0
 F16 = 1
 BF16 = 2                   # rows of the operators below only
+MX4 = 4                    # storage type of IndexFlat only: microscaled 4-bit floating point
 
 _lib = None
 
@@ -75,6 +76,8 @@ def load() -> C.CDLL:
         "b200idx_merge_topk_device": (i32, [i32, i64, i32, i32, vp, vp, vp, vp, vp]),
         "b200idx_merge_topk_device_strided": (i32, [i32, i64, i32, i32, vp, vp, i64, vp, vp, vp]),
         "b200idx_rms_norm_i8_device": (i32, [i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, vp, i64, vp, vp]),
+        "b200idx_add_states_device": (i32, [vp, i64, i32, vp, vp, vp, C.c_float, vp, vp]),
+        "b200idx_search_states_device": (i32, [vp, i64, i32, vp, vp, vp, C.c_float, vp, i32, vp, vp]),
         "b200idx_i8_dequantize_device": (i32, [i64, i32, vp, i64, vp, vp, i32, vp, i64, vp]),
         "b200idx_mx4_row_bytes": (i64, [i32]),
         "b200idx_mx4_scale_bytes": (i64, [i64, i32]),
@@ -130,7 +133,7 @@ EXPORTED_SYMBOLS = [
     "b200idx_ivfpq_search_preassigned_device", "b200idx_ivfpq_get_nprobe", "b200idx_ivfpq_list_length",
     "b200idx_ivfpq_get_list", "b200idx_stats", "b200idx_set_timing", "b200idx_stream", "b200idx_last_error",
     "b200idx_status_of_message",
-    "b200idx_rms_norm_i8_device", "b200idx_i8_dequantize_device", "b200idx_mx4_row_bytes", "b200idx_mx4_scale_bytes",
+    "b200idx_rms_norm_i8_device", "b200idx_add_states_device", "b200idx_search_states_device", "b200idx_i8_dequantize_device", "b200idx_mx4_row_bytes", "b200idx_mx4_scale_bytes",
     "b200idx_mx4_quantize_device", "b200idx_mx4_dequantize_device", "b200idx_mx4_product_device",
     "b200idx_version",
 ]
@@ -261,7 +264,7 @@ class _Index:
 
 
 class IndexFlat(_Index):
-    """Exact search, fp32 (default) or fp16 rows -- mirror of ``faiss::ascend::AscendIndexFlat``
+    """Exact search, fp32 (default), fp16 or MX4 rows -- mirror of ``faiss::ascend::AscendIndexFlat``
     (feature_retrieval/src/ascendfaiss/ascend/AscendIndexFlat.h:48-90) on one device."""
 
     def __init__(self, d: int, metric: int = METRIC_L2, dtype: int = F32, device: int = 0):
@@ -284,7 +287,7 @@ class IndexFlat(_Index):
 
     def get_base(self, offset: int = 0, n: int | None = None):
         n = self.ntotal - offset if n is None else n
-        out = np.empty((n, self.d), np.float32 if self.dtype == F32 else np.uint16)
+        out = np.empty((n, self.d), np.uint16 if self.dtype == F16 else np.float32)
         _check(self._lib.b200idx_get_base(self._h, offset, n, _ptr(out)), self._h)
         return out
 
@@ -304,6 +307,19 @@ class IndexInt8Flat(_Index):
         super().__init__()
         self.metric = metric
         _check(self._lib.b200idx_create_int8flat(d, metric, device, C.byref(self._h)))
+
+    def add_states_device(self, n: int, dtype: int, x_ptr: int, weight_ptr: int, eps: float, *, residual_ptr: int = 0,
+                          static_scale_ptr: int = 0, ids=None):
+        """Adds the rows that rms_norm_i8_device makes of n hidden states on the index's device."""
+        idp = None if ids is None else np.ascontiguousarray(ids, dtype=np.int64)
+        _check(self._lib.b200idx_add_states_device(self._h, n, dtype, x_ptr, residual_ptr, weight_ptr, eps,
+                                                   static_scale_ptr, _ptr(idp)), self._h)
+
+    def search_states_device(self, n: int, dtype: int, x_ptr: int, weight_ptr: int, eps: float, k: int, D_ptr: int,
+                             I_ptr: int, *, residual_ptr: int = 0, static_scale_ptr: int = 0):
+        """Searches for the rows that rms_norm_i8_device makes of n hidden states on the index's device."""
+        _check(self._lib.b200idx_search_states_device(self._h, n, dtype, x_ptr, residual_ptr, weight_ptr, eps,
+                                                      static_scale_ptr, k, D_ptr, I_ptr), self._h)
 
     def get_base(self, offset: int = 0, n: int | None = None):
         n = self.ntotal - offset if n is None else n
@@ -411,7 +427,7 @@ def load_index(path: str, device: int = 0):
     if kind == 0:
         ix = IndexFlat.__new__(IndexFlat)
         _Index.__init__(ix)
-        ix.metric, ix.dtype = metric, (F16 if dtype == 1 else F32)
+        ix.metric, ix.dtype = metric, {1: F16, 4: MX4}.get(dtype, F32)
     elif kind == 1:
         ix = IndexInt8Flat.__new__(IndexInt8Flat)
         _Index.__init__(ix)

@@ -146,10 +146,11 @@ extern "C" {
 int b200idx_create_flat(int d, int metric, int dtype, int device, b200idx_t** out) {
     return guarded_create([&] {
         check_common_create(d, metric, device, out);
-        if (dtype != B200IDX_F32 && dtype != B200IDX_F16) throw std::invalid_argument("Unsupported dtype");
+        if (dtype != B200IDX_F32 && dtype != B200IDX_F16 && dtype != B200IDX_MX4)
+            throw std::invalid_argument("Unsupported dtype");
         std::unique_ptr<b200idx_index> h(new b200idx_index);
         h->kind = 0;
-        h->flat.reset(new FlatIndex(d, metric, dtype == B200IDX_F32 ? kF32 : kF16, device));
+        h->flat.reset(new FlatIndex(d, metric, dtype == B200IDX_F32 ? kF32 : (dtype == B200IDX_F16 ? kF16 : kMX4), device));
         *out = h.release();
     });
 }
@@ -572,7 +573,8 @@ int b200idx_ivfpq_get_list(const b200idx_t* h, int list, uint8_t* codes, int64_t
 // ---------------------------------------------------------------------------------------
 // Native file format (little-endian):
 //   "B2IX" | u32 version = 1 | u32 kind (0 Flat, 1 Int8Flat, 2 IVFPQ) | i32 d | i32 metric | i32 dtype | i64 ntotal
-//   Flat / Int8Flat : ntotal rows in the index's storage dtype (fp32, fp16 or int8) | ntotal int64 labels
+//   Flat / Int8Flat : ntotal rows in the index's storage dtype (fp32, fp16, int8; MX4: a row's codes and then its
+//                     scale bytes) | ntotal int64 labels
 //   IVFPQ           : i32 nlist | i32 M | i32 nbits | i32 by_residual | i32 nprobe | i32 trained |
 //                     centroids [nlist][d] fp32 | codebooks [M][256][d/M] fp32 |
 //                     per list: i64 length | codes [length][M] (canonical byte order) | ids [length]
@@ -612,13 +614,15 @@ int b200idx_save(const b200idx_t* h, const char* path) {
             put_v<int32_t>(f.get(), ix.metric());
             put_v<int32_t>(f.get(), ix.dtype());
             put_v<int64_t>(f.get(), ix.ntotal());
-            const size_t row = static_cast<size_t>(ix.d()) * storage_elem_bytes(ix.dtype());
+            const bool mx4 = ix.dtype() == kMX4;
+            const size_t row = mx4 ? ix.mx4_file_row() : static_cast<size_t>(ix.d()) * storage_elem_bytes(ix.dtype());
             const int64_t chunk = std::max<int64_t>(1, (int64_t(64) << 20) / static_cast<int64_t>(row));
             std::vector<uint8_t> buf;
             for (int64_t o = 0; o < ix.ntotal(); o += chunk) {
                 const int64_t m = std::min(chunk, ix.ntotal() - o);
                 buf.resize(static_cast<size_t>(m) * row);
-                ix.get_base(o, m, buf.data());
+                if (mx4) ix.get_mx4_rows(o, m, buf.data());
+                else ix.get_base(o, m, buf.data());
                 put(f.get(), buf.data(), buf.size());
             }
             std::vector<int64_t> ids(static_cast<size_t>(ix.ntotal()));
@@ -677,7 +681,7 @@ int b200idx_load(const char* path, int device, b200idx_t** out) {
         const int64_t ntotal = get_v<int64_t>(f.get());
         if (kind > 2 || ntotal < 0) throw std::invalid_argument("corrupt index file");
         int rc;
-        if (kind == 0) rc = b200idx_create_flat(d, metric, dtype == kF16 ? B200IDX_F16 : B200IDX_F32, device, &h);
+        if (kind == 0) rc = b200idx_create_flat(d, metric, dtype == kF16 ? B200IDX_F16 : (dtype == kMX4 ? B200IDX_MX4 : B200IDX_F32), device, &h);
         else if (kind == 1) rc = b200idx_create_int8flat(d, metric, device, &h);
         else {
             const int nlist = get_v<int32_t>(f.get()), M = get_v<int32_t>(f.get()), nbits = get_v<int32_t>(f.get());
@@ -686,7 +690,8 @@ int b200idx_load(const char* path, int device, b200idx_t** out) {
         }
         if (rc != B200IDX_OK) throw std::invalid_argument(std::string("corrupt index file: ") + b200idx_last_error(nullptr));
         if (kind != 2) {
-            const size_t row = static_cast<size_t>(d) * storage_elem_bytes(h->flat->dtype());
+            const bool mx4 = h->flat->dtype() == kMX4;
+            const size_t row = mx4 ? h->flat->mx4_file_row() : static_cast<size_t>(d) * storage_elem_bytes(h->flat->dtype());
             const int64_t chunk = std::max<int64_t>(1, (int64_t(64) << 20) / static_cast<int64_t>(row));
             std::vector<uint8_t> rows(static_cast<size_t>(std::min<int64_t>(chunk, std::max<int64_t>(ntotal, 1))) * row);
             // labels follow the rows: read them first
@@ -699,7 +704,8 @@ int b200idx_load(const char* path, int device, b200idx_t** out) {
             for (int64_t o = 0; o < ntotal; o += chunk) {
                 const int64_t m = std::min(chunk, ntotal - o);
                 get(f.get(), rows.data(), static_cast<size_t>(m) * row);
-                h->flat->add(m, rows.data(), h->flat->dtype() == kF16, ids.data() + o, false);
+                if (mx4) h->flat->add_mx4_rows(m, rows.data(), ids.data() + o);
+                else h->flat->add(m, rows.data(), h->flat->dtype() == kF16, ids.data() + o, false);
             }
         } else {
             IvfpqIndex& ix = *h->ivfpq;

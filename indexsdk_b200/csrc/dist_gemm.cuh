@@ -17,7 +17,7 @@ constexpr int kTileQ = 128;   // query rows per accumulator tile (TMEM lanes)
 constexpr int kTileB = 256;   // base rows per accumulator tile (TMEM columns)
 constexpr int kChunkBytes = 128;  // K extent of one pipeline stage, in bytes (one 128-byte swizzle row)
 
-enum GemmKind : int { kKindF16 = 0, kKindBF16 = 1, kKindI8 = 2 };
+enum GemmKind : int { kKindF16 = 0, kKindBF16 = 1, kKindI8 = 2, kKindMX4 = 16 };   // (MX4: mx4_gemm.cuh)
 
 // bf16 operands are "folded": every row carries kFoldCols extra K columns so that the tensor core
 // itself adds the base norm and the query's threshold to the dot product,

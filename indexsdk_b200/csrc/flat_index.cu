@@ -9,6 +9,7 @@
 #include <unordered_set>
 
 #include "dist_gemm.cuh"
+#include "mx4_gemm.cuh"
 #include "select.cuh"
 
 namespace b200 {
@@ -76,7 +77,13 @@ FlatIndex::~FlatIndex() {
 }
 
 int FlatIndex::gemm_kind() const {
+    if (dtype_ == kMX4) return kKindMX4;
     return dtype_ == kI8 ? kKindI8 : (dtype_ == kF16 ? kKindF16 : kKindBF16);
+}
+
+cudaError_t FlatIndex::launch_gemm(const GemmLaunch& L, const GemmArgs& a, const CUtensorMap* map_a) {
+    if (dtype_ == kMX4) return launch_mx4_dist(L, a, w_qsc_.as<uint8_t>(), xsc_.as<uint8_t>(), map_a, &map_b_, stream_);
+    return launch_dist_gemm(L, a, map_a, &map_b_, stream_);
 }
 
 void FlatIndex::reserve(int64_t n) {
@@ -86,7 +93,9 @@ void FlatIndex::reserve(int64_t n) {
     map_b_valid_ = false;
     int64_t want = std::max<int64_t>(n, cap_rows_ + cap_rows_ / 2);
     want = round_up(want, kTileB);
-    const size_t row_op = static_cast<size_t>(op_cols()) * op_elem_bytes();
+    const size_t row_op = op_row_bytes();
+    if (dtype_ == kMX4)
+        xsc_.grow_keep(static_cast<size_t>(mx4_scale_bytes(want, d_)), n_ ? static_cast<size_t>(mx4_scale_bytes(n_, d_)) : 0, stream_);
     if (dtype_ == kF32)
         x32_.grow_keep(static_cast<size_t>(want) * d_ * 4, static_cast<size_t>(n_) * d_ * 4, stream_);
     // whole tiles are kept: a packed operand copy interleaves the rows of a tile
@@ -96,11 +105,15 @@ void FlatIndex::reserve(int64_t n) {
     cap_rows_ = want;
 }
 
+void FlatIndex::begin_add(int64_t n) {
+    if (n_ + n > 0xFFFFFFF0ll) throw std::invalid_argument("a single-device index holds at most 2^32 - 16 vectors");
+    reserve(n_ + n);
+}
+
 void FlatIndex::add(int64_t n, const void* x, bool x_is_f16, const int64_t* ids, bool x_on_device) {
     if (n <= 0) return;
     DeviceGuard g(device_);
-    if (n_ + n > 0xFFFFFFF0ll) throw std::invalid_argument("a single-device index holds at most 2^32 - 16 vectors");
-    reserve(n_ + n);
+    begin_add(n);
     const cudaMemcpyKind kind = x_on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
     const size_t rows_per_chunk = std::max<size_t>(1, (size_t(256) << 20) / (static_cast<size_t>(d_) * 4));
     for (int64_t off = 0; off < n; off += static_cast<int64_t>(rows_per_chunk)) {
@@ -124,6 +137,15 @@ void FlatIndex::add(int64_t n, const void* x, bool x_is_f16, const int64_t* ids,
                 B200_CUDA_CHECK(launch_f32_to_f16(st, m * d_, dst, stream_));
             }
             B200_CUDA_CHECK(launch_base_prep_f16(dst, m, d_, norms_.as<float>() + row0, stream_));
+        } else if (dtype_ == kMX4) {
+            const float* src = static_cast<const float*>(x) + off * d_;
+            if (!x_on_device) {
+                float* st = static_cast<float*>(w_stage_in_.ensure(static_cast<size_t>(m) * d_ * 4));
+                B200_CUDA_CHECK(cudaMemcpyAsync(st, src, static_cast<size_t>(m) * d_ * 4, kind, stream_));
+                src = st;
+            }
+            B200_CUDA_CHECK(launch_mx4_quantize(kF32, m, d_, src, d_, row0, xop_.as<uint8_t>(), xsc_.as<uint8_t>(),
+                                                norms_.as<float>(), stream_));
         } else {
             int8_t* dst = xop_.as<int8_t>() + row0 * d_;
             B200_CUDA_CHECK(cudaMemcpyAsync(dst, static_cast<const int8_t*>(x) + off * d_,
@@ -132,6 +154,11 @@ void FlatIndex::add(int64_t n, const void* x, bool x_is_f16, const int64_t* ids,
         }
         B200_CUDA_CHECK(cudaStreamSynchronize(stream_));  // staging buffer and user memory are reusable
     }
+    finish_add(n, ids);
+}
+
+// The n rows behind the last one are in place (queued): labels, then they count.
+void FlatIndex::finish_add(int64_t n, const int64_t* ids) {
     if (ids) {
         B200_CUDA_CHECK(cudaMemcpyAsync(labels_.as<int64_t>() + n_, ids, static_cast<size_t>(n) * 8,
                                         cudaMemcpyDefault, stream_));
@@ -148,6 +175,55 @@ void FlatIndex::add(int64_t n, const void* x, bool x_is_f16, const int64_t* ids,
     n_ += n;
     generation_ = next_generation();
     map_b_valid_ = false;
+}
+
+void FlatIndex::add_states(int64_t n, int states_dtype, RmsNormArgs a, const int64_t* ids) {
+    DeviceGuard g(device_);
+    begin_add(n);
+    a.n = n;
+    a.d = d_;
+    a.q = xop_.as<int8_t>() + n_ * d_;
+    a.ldq = d_;
+    if (!a.static_scale) a.scales = static_cast<float*>(w_state_s_.ensure(static_cast<size_t>(n) * 4));
+    B200_CUDA_CHECK(launch_rms_norm_i8(states_dtype, a, stream_));
+    B200_CUDA_CHECK(launch_base_prep_i8(a.q, n, d_, norms_.as<int32_t>() + n_, stream_));
+    finish_add(n, ids);
+}
+
+void FlatIndex::search_states(int64_t nq, int states_dtype, RmsNormArgs a, int k, float* D, int64_t* I) {
+    DeviceGuard g(device_);
+    a.n = nq;
+    a.d = d_;
+    a.q = static_cast<int8_t*>(w_state_q_.ensure(static_cast<size_t>(nq) * d_));
+    a.ldq = d_;
+    if (!a.static_scale) a.scales = static_cast<float*>(w_state_s_.ensure(static_cast<size_t>(nq) * 4));
+    B200_CUDA_CHECK(launch_rms_norm_i8(states_dtype, a, stream_));
+    stats_.kernel_launches += 1;
+    search_device(nq, a.q, false, k, D, I, k);
+}
+
+size_t FlatIndex::mx4_file_row() const { return static_cast<size_t>(mx4_pitch(d_)) + mx4_blocks(d_); }
+
+void FlatIndex::get_mx4_rows(int64_t offset, int64_t n, uint8_t* out) const {
+    if (n <= 0) return;
+    DeviceGuard g(device_);
+    if (offset < 0 || offset + n > n_) throw std::invalid_argument("get_mx4_rows: range outside the index");
+    DeviceBuffer tmp;
+    uint8_t* t = static_cast<uint8_t*>(tmp.ensure(static_cast<size_t>(n) * mx4_file_row()));
+    B200_CUDA_CHECK(launch_mx4_pack_rows(n, d_, offset, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), t, true, stream_));
+    B200_CUDA_CHECK(cudaMemcpyAsync(out, t, static_cast<size_t>(n) * mx4_file_row(), cudaMemcpyDeviceToHost, stream_));
+    B200_CUDA_CHECK(cudaStreamSynchronize(stream_));
+}
+
+void FlatIndex::add_mx4_rows(int64_t n, const uint8_t* rows, const int64_t* ids) {
+    if (n <= 0) return;
+    DeviceGuard g(device_);
+    begin_add(n);
+    uint8_t* t = static_cast<uint8_t*>(w_stage_in_.ensure(static_cast<size_t>(n) * mx4_file_row()));
+    B200_CUDA_CHECK(cudaMemcpyAsync(t, rows, static_cast<size_t>(n) * mx4_file_row(), cudaMemcpyHostToDevice, stream_));
+    B200_CUDA_CHECK(launch_mx4_pack_rows(n, d_, n_, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), t, false, stream_));
+    B200_CUDA_CHECK(launch_mx4_norms(n, d_, n_, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), norms_.as<float>(), stream_));
+    finish_add(n, ids);
 }
 
 void FlatIndex::reset() {
@@ -171,7 +247,7 @@ int64_t FlatIndex::remove_ids(int64_t n, const int64_t* ids) {
         if (rm.count(lab[static_cast<size_t>(i)])) pos.push_back(i);
     // Swap-with-last compaction, highest position first, as the reference's removeIds does
     // (FR/ascenddaemon/impl/Index.cpp:86-140).
-    const size_t row_op = static_cast<size_t>(op_cols()) * op_elem_bytes();
+    const size_t row_op = op_row_bytes();
     const size_t norm_b = 4;
     int64_t last = n_ - 1;
     for (auto it = pos.rbegin(); it != pos.rend(); ++it, --last) {
@@ -186,6 +262,7 @@ int64_t FlatIndex::remove_ids(int64_t n, const int64_t* ids) {
         else
             B200_CUDA_CHECK(cudaMemcpyAsync(xop_.as<uint8_t>() + p * row_op, xop_.as<uint8_t>() + last * row_op, row_op,
                                             cudaMemcpyDeviceToDevice, stream_));
+        if (dtype_ == kMX4) B200_CUDA_CHECK(launch_mx4_move_scales(d_, last, p, xsc_.as<uint8_t>(), stream_));
         B200_CUDA_CHECK(cudaMemcpyAsync(norms_.as<uint8_t>() + p * norm_b, norms_.as<uint8_t>() + last * norm_b,
                                         norm_b, cudaMemcpyDeviceToDevice, stream_));
         B200_CUDA_CHECK(cudaMemcpyAsync(labels_.as<int64_t>() + p, labels_.as<int64_t>() + last, 8,
@@ -202,6 +279,18 @@ void FlatIndex::get_base(int64_t offset, int64_t n, void* out) const {
     if (n <= 0) return;
     DeviceGuard g(device_);
     if (offset < 0 || offset + n > n_) throw std::invalid_argument("get_base: range outside the index");
+    if (dtype_ == kMX4) {   // the values that the rows stand for
+        DeviceBuffer tmp;
+        const int64_t page = std::max<int64_t>(1, (int64_t(64) << 20) / (static_cast<int64_t>(d_) * 4));
+        float* t = static_cast<float*>(tmp.ensure(static_cast<size_t>(std::min(page, n)) * d_ * 4));
+        for (int64_t o = 0; o < n; o += page) {
+            const int64_t m = std::min(page, n - o);
+            B200_CUDA_CHECK(launch_mx4_dequantize(offset + o, m, d_, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), kF32, t, d_, stream_));
+            B200_CUDA_CHECK(cudaMemcpyAsync(static_cast<float*>(out) + o * d_, t, static_cast<size_t>(m) * d_ * 4, cudaMemcpyDeviceToHost, stream_));
+            B200_CUDA_CHECK(cudaStreamSynchronize(stream_));
+        }
+        return;
+    }
     if (dtype_ == kF32)
         B200_CUDA_CHECK(cudaMemcpy(out, x32_.as<float>() + offset * d_, static_cast<size_t>(n) * d_ * 4,
                                    cudaMemcpyDeviceToHost));
@@ -305,6 +394,11 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
         xq_op = qop;
     } else if (dtype_ == kF16) {
         B200_CUDA_CHECK(launch_prep_queries_f16(xq_raw, nq, d_, static_cast<float*>(qnorm), stream_));
+    } else if (dtype_ == kMX4) {
+        uint8_t* qop = static_cast<uint8_t*>(w_qop_.ensure(static_cast<size_t>(nq) * op_row_bytes()));
+        uint8_t* qsc = static_cast<uint8_t*>(w_qsc_.ensure(static_cast<size_t>(mx4_scale_bytes(nq, d_))));
+        B200_CUDA_CHECK(launch_mx4_quantize(kF32, nq, d_, xq_raw, d_, 0, qop, qsc, static_cast<float*>(qnorm), stream_));
+        xq_op = qop;
     } else {
         B200_CUDA_CHECK(launch_prep_queries_i8(static_cast<const int8_t*>(xq_raw), nq, d_,
                                                static_cast<int32_t*>(qnorm), stream_));
@@ -313,7 +407,15 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
 
     // 2. operand maps
     CUtensorMap map_a;
-    if (!use_simt_) {
+    if (dtype_ == kMX4) {   // (no CUDA-core variant)
+        if (!map_b_valid_) {
+            if (encode_mx4_map(&map_b_, xop_.as<uint8_t>(), n_, d_, kTileB) != 0)
+                throw std::runtime_error("cuTensorMapEncodeTiled failed for the base operand");
+            map_b_valid_ = true;
+        }
+        if (encode_mx4_map(&map_a, static_cast<const uint8_t*>(xq_op), nq, d_, kTileQ) != 0)
+            throw std::runtime_error("cuTensorMapEncodeTiled failed for the query operand");
+    } else if (!use_simt_) {
         if (!map_b_valid_) {
             if (encode_operand_map(&map_b_, kind, xop_.get(), n_, op_cols(), kTileB) != 0)
                 throw std::runtime_error("cuTensorMapEncodeTiled failed for the base operand");
@@ -375,7 +477,7 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
         L.mode = kModeBurstMin;
         L.burst = plan.burst;
         a.prof = prof_ ? w_prof_.as<unsigned long long>() : nullptr;
-        B200_CUDA_CHECK(launch_dist_gemm(L, a, &map_a, &map_b_, stream_));
+        B200_CUDA_CHECK(launch_gemm(L, a, &map_a));
         fold.counts = counts;
         B200_CUDA_CHECK(launch_kth_threshold(mins, stride, stride, nq, k, eps, tau_all, tau, fold, stream_));
         fold.counts = nullptr;
@@ -407,7 +509,7 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
     int first_stretch = two_stretches ? std::max(n_tiles / 5, 2 * plan.s_tiles) : n_tiles;
     a.tile_first = 0;
     a.n_tiles_sel = first_stretch;
-    B200_CUDA_CHECK(launch_dist_gemm(L, a, &map_a, &map_b_, stream_));
+    B200_CUDA_CHECK(launch_gemm(L, a, &map_a));
     stats_.gemm_launches += 1;
     stats_.kernel_launches += 1;
     auto report_counts = [&](const char* what) {   // development aid (B200IDX_PROF=1)
@@ -429,7 +531,7 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
 #ifdef B200IDX_DEV_PROF
         if (prof_ && getenv("B200IDX_GEMM_TRACE")) a.trace = w_prof_.as<unsigned long long>() + 32;
 #endif
-        B200_CUDA_CHECK(launch_dist_gemm(L, a, &map_a, &map_b_, stream_));
+        B200_CUDA_CHECK(launch_gemm(L, a, &map_a));
         a.trace = nullptr;
         stats_.gemm_launches += 1;
         stats_.kernel_launches += 2;

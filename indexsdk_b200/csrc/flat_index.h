@@ -6,6 +6,7 @@
 // 262144-row blocks and no fractal layouts.
 #pragma once
 #include "dist_gemm.cuh"
+#include "row_ops.cuh"
 #include "select.cuh"
 #include <cuda.h>
 #include <stdint.h>
@@ -93,7 +94,8 @@ private:
 class FlatIndex {
 public:
     // dtype: kF32 (fp32 rows + bf16 filter copy, results refined in fp32), kF16 (fp16 rows,
-    // fp32 accumulation, results are the GEMM's), kI8 (int8 rows, exact int32).
+    // fp32 accumulation, results are the GEMM's), kI8 (int8 rows, exact int32), kMX4 (float rows in, kept as
+    // microscaled 4-bit codes and scales; queries are rounded the same way; results are the GEMM's).
     FlatIndex(int d, int metric, int dtype, int device);
     ~FlatIndex();
 
@@ -111,11 +113,19 @@ public:
     // x: host or device pointer in the index's input dtype (float for kF32 and kF16 unless
     // x_is_f16, int8 for kI8).  ids: host pointer or nullptr (labels = ntotal + i).
     void add(int64_t n, const void* x, bool x_is_f16, const int64_t* ids, bool x_on_device);
+    // Int8 rows from hidden states on the device: residual addition, RMS norm and rounding (a.n, a.d, a.q and
+    // a.scales are filled in here).
+    void add_states(int64_t n, int states_dtype, RmsNormArgs a, const int64_t* ids);
+    void search_states(int64_t nq, int states_dtype, RmsNormArgs a, int k, float* D, int64_t* I);
     void reset();
     int64_t remove_ids(int64_t n, const int64_t* ids);
     // Copies rows [offset, offset + n) to a host buffer: float for kF32, fp16 bits for kF16,
     // int8 for kI8.
     void get_base(int64_t offset, int64_t n, void* out_host) const;
+    // kMX4: rows as they are stored, per row its codes and then its scale bytes; and back.
+    size_t mx4_file_row() const;
+    void get_mx4_rows(int64_t offset, int64_t n, uint8_t* out_host) const;
+    void add_mx4_rows(int64_t n, const uint8_t* rows_host, const int64_t* ids);
     void get_labels(int64_t offset, int64_t n, int64_t* out_host) const;
 
     // Device-resident search.  xq: device pointer, rows of float (kF32, kF16 unless q_is_f16) or
@@ -174,6 +184,11 @@ private:
     PageTail run_page(int nq, const void* xq_raw, const void* xq_op, int k, float* D, int64_t* I, int ldk,
                   const int32_t* qmap_dev, bool force_full);
     void reserve(int64_t n);
+    void begin_add(int64_t n);
+    void finish_add(int64_t n, const int64_t* ids);
+    cudaError_t launch_gemm(const GemmLaunch& L, const GemmArgs& a, const CUtensorMap* map_a);
+    // bytes of a row of xop_
+    size_t op_row_bytes() const { return dtype_ == kMX4 ? static_cast<size_t>(mx4_pitch(d_)) : static_cast<size_t>(op_cols()) * op_elem_bytes(); }
     size_t in_elem_bytes() const { return dtype_ == kI8 ? 1 : (dtype_ == kF16 ? 2 : 4); }
     size_t op_elem_bytes() const { return dtype_ == kI8 ? 1 : 2; }
   public:
@@ -201,7 +216,8 @@ private:
     const uint32_t* mask_cur_ = nullptr;
     int64_t mask_stride_ = 0;
     DeviceBuffer w_mask_, w_fb_mask_;
-    DeviceBuffer xop_;     // GEMM operand rows: bf16 (kF32), fp16 (kF16), int8 (kI8)
+    DeviceBuffer xop_;     // GEMM operand rows: bf16 (kF32), fp16 (kF16), int8 (kI8), codes (kMX4)
+    DeviceBuffer xsc_;     // kMX4: scales, whole blocks of 128 rows
     DeviceBuffer norms_;   // float (kF32/kF16) or int32 (kI8), padded to a multiple of 256 rows
     DeviceBuffer labels_;  // int64 per row
     DeviceBuffer maxnorm_; // float: max squared base norm (kF32)
@@ -210,6 +226,7 @@ private:
     CUtensorMap map_b_;
 
     // scratch
+    DeviceBuffer w_qsc_, w_state_q_, w_state_s_;
     DeviceBuffer w_qop_, w_qraw_, w_qnorm_, w_eps_, w_mins_, w_tau_, w_cand_, w_counts_, w_qmap_,
         w_err_, w_stage_in_, w_stage_D_, w_stage_I_, w_fb_q_, w_fb_qop_, w_prof_;
     bool prof_ = false;

@@ -36,6 +36,7 @@ __global__ void gather_members_kernel(const MemberView* members, const int32_t* 
 
 bool FlatGroup::eligible(const std::vector<FlatIndex*>& m, int64_t nq, int k) {
     if (m.size() < 2 || nq <= 0 || nq > 0x7FFFFFFF / static_cast<int64_t>(m.size())) return false;
+    if (m[0]->dtype() == kMX4) return false;   // (searched one after the other)
     int64_t cap = 0, total = 0;
     for (const FlatIndex* ix : m) {
         if (ix->ntotal() <= 0 || ix->ntotal() > kMaxMemberRows) return false;

@@ -72,6 +72,7 @@ extern "C" int b200idx_search_device_noalloc(b200idx_t* h, int64_t n, const void
     return b200_capi::guarded(h, [&] {
         FlatIndex* ix = b200_capi::flat_of(h);
         if (!ix) throw std::invalid_argument("the no-allocation search applies to Flat and Int8Flat indexes");
+        if (ix->dtype() == kMX4) throw std::invalid_argument("the no-allocation search does not apply to MX4 indexes");
         if (n <= 0 || !x_dev || !D_dev || !I_dev) throw std::invalid_argument("n must be > 0, pointers non-NULL");
         if (k <= 0 || k > kMaxKNoAlloc) throw std::invalid_argument("k must be in [1, 1024] for the no-allocation search");
         const FlatIndex::RawView v = ix->raw_view();

@@ -34,6 +34,10 @@ int64_t stride(int64_t ld, int d, const char* what) {
     return ld;
 }
 
+void check_eps(float eps) {
+    if (!(eps >= 1e-12f && eps <= 1.f)) throw std::invalid_argument("eps must be in [1e-12, 1]");
+}
+
 struct Operand {
     const char* name;
     const void* p;
@@ -66,6 +70,32 @@ int device_of(std::initializer_list<Operand> ops) {
     return device;
 }
 
+FlatIndex* states_index(b200idx_t* h) {
+    FlatIndex* ix = b200_capi::flat_of(h);
+    if (!ix || ix->dtype() != kI8) throw std::invalid_argument("states are accepted by Int8Flat indexes only");
+    return ix;
+}
+RmsNormArgs states_args(const FlatIndex* ix, int64_t n, int dtype, const void* x, const void* residual,
+                        const void* weight, float eps, const float* static_scale) {
+    check_rows(n, "n");
+    const size_t eb = elem_bytes(dtype);
+    check_eps(eps);
+    if (!static_scale && ix->metric() != kMetricCos)
+        throw std::invalid_argument("inner products and L2 distances need a static_scale: rows with scales of their own do not compare");
+    const Operand xo{"x", x, eb};
+    if (device_of({xo, {"weight", weight, eb}, residual ? Operand{"residual", residual, eb} : xo,
+                   static_scale ? Operand{"static_scale", static_scale, 4} : xo}) != ix->device())
+        throw std::invalid_argument("the states must lie on the index's device");
+    RmsNormArgs a{};
+    a.x = x;
+    a.ldx = a.ldr = ix->d();
+    a.residual = residual;
+    a.weight = weight;
+    a.eps = eps;
+    a.static_scale = static_scale;
+    return a;
+}
+
 int sm_count(int device) {
     int sms = 0;
     B200_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
@@ -83,18 +113,41 @@ int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64
         check_rows(n, "n");
         check_dim(d);
         const size_t eb = elem_bytes(dtype);
-        if (!(eps >= 1e-12f && eps <= 1.f)) throw std::invalid_argument("eps must be in [1e-12, 1]");
-        if (!residual != !sum) throw std::invalid_argument("residual and sum go together: give both or neither");
+        check_eps(eps);
+        if (sum && !residual) throw std::invalid_argument("a sum needs a residual");
         if (!static_scale == !scales) throw std::invalid_argument("give exactly one of static_scale and scales");
         RmsNormArgs a{n, d, x, stride(ldx, d, "ldx"), residual, stride(ldr, d, "ldr"), sum, stride(lds, d, "lds"),
                       weight, eps, static_scale, q, stride(ldq, d, "ldq"), scales};
-        if (residual && ((sum == x && a.lds != a.ldx) || (sum == residual && a.lds != a.ldr)))
+        if (sum && ((sum == x && a.lds != a.ldx) || (sum == residual && a.lds != a.ldr)))
             throw std::invalid_argument("sum in place of x or residual needs the same stride");
         const float* sc = static_scale ? static_scale : scales;
         const Operand no{"q", q, 1};   // (repeats a required one where the optional ones are absent)
         DeviceGuard g(device_of({{"x", x, eb}, {"weight", weight, eb}, no, {"scales", sc, 4},
                                  residual ? Operand{"residual", residual, eb} : no, sum ? Operand{"sum", sum, eb} : no}));
         B200_CUDA_CHECK(launch_rms_norm_i8(dtype, a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int b200idx_add_states_device(b200idx_t* h, int64_t n, int dtype, const void* x, const void* residual, const void* weight,
+                              float eps, const float* static_scale, const int64_t* ids_host) {
+    if (!h) return B200IDX_ERR_INVALID_PARAM;
+    return b200_capi::guarded(h, [&] {
+        FlatIndex* ix = states_index(h);
+        const RmsNormArgs a = states_args(ix, n, dtype, x, residual, weight, eps, static_scale);
+        ix->add_states(n, dtype, a, ids_host);
+    });
+}
+
+int b200idx_search_states_device(b200idx_t* h, int64_t n, int dtype, const void* x, const void* residual,
+                                 const void* weight, float eps, const float* static_scale, int k, float* distances,
+                                 int64_t* labels) {
+    if (!h) return B200IDX_ERR_INVALID_PARAM;
+    return b200_capi::guarded(h, [&] {
+        FlatIndex* ix = states_index(h);
+        const RmsNormArgs a = states_args(ix, n, dtype, x, residual, weight, eps, static_scale);
+        if (k <= 0 || k > 4096) throw std::invalid_argument("k must be > 0 and <= 4096");
+        device_of({{"distances", distances, 4}, {"labels", labels, 8}});
+        ix->search_states(n, dtype, a, k, distances, labels);
     });
 }
 

@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) rms_norm_i8_kernel(const 
                 // model carries on, so the result is that of the two steps done one after the other.
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[j][e] = to_f<T>(from_f<T>(v[j][e] + f[j][e]));
+                if (!a.sum) continue;
                 if (whole(j)) {
                     store8<T>(sum_row + at(j, 0), v[j]);
                 } else {
@@ -137,14 +138,20 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) rms_norm_i8_kernel(const 
         reduce_row<NT>(ssq, top, sh);
         if (!(ssq <= 3.4e38f) || !(top <= 3.4e38f)) {
             // The squares left the range of fp32 (or the row holds no numbers): once more with values scaled by
-            // 2^-100, from what this thread itself wrote or did not touch.
+            // 2^-100.  The sum may have taken x's or the residual's place; this thread wrote what it reads.
             pre = 7.8886090522101181e-31f;
             ssq = top = 0.f;
-            const T* again = a.residual ? sum_row : x;
+            const T* again = a.sum ? sum_row : x;
+            const T* r = a.residual && !a.sum ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 float w[8];
                 fetch(again, j, v[j]);
+                if (r) {
+                    fetch(r, j, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] = to_f<T>(from_f<T>(v[j][e] + w[e]));
+                }
                 fetch(weight, j, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -371,6 +378,57 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(int64_t row0, int64
     }
 }
 
+__global__ void mx4_move_scales_kernel(int ng, int64_t from, int64_t to, uint8_t* scales) {
+    for (int g = threadIdx.x; g < ng; g += blockDim.x)
+        *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(to, g, ng)) = *reinterpret_cast<const uint32_t*>(scales + mx4_scale_word(from, g, ng));
+}
+
+// A warp per row.
+__global__ void __launch_bounds__(256) mx4_pack_rows_kernel(int64_t n, int d, int64_t row0, uint8_t* codes, uint8_t* scales,
+                                                            uint8_t* plain, int out) {
+    const int nb = mx4_blocks(d), ng = mx4_groups(d), lane = threadIdx.x & 31;
+    const int64_t pitch = mx4_pitch(d);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < n; r += static_cast<int64_t>(gridDim.x) * 8) {
+        uint8_t* c = codes + (row0 + r) * pitch;
+        uint8_t* p = plain + r * (pitch + nb);
+        for (int i = lane; i < pitch; i += 32) {
+            if (out) p[i] = c[i];
+            else c[i] = p[i];
+        }
+        for (int b = lane; b < 4 * ng; b += 32) {
+            uint8_t* s = scales + mx4_scale_word(row0 + r, b >> 2, ng) + (b & 3);
+            if (!out) *s = b < nb ? p[pitch + b] : 127;
+            else if (b < nb) p[pitch + b] = *s;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) mx4_norms_kernel(int64_t n, int d, int64_t row0, const uint8_t* codes,
+                                                        const uint8_t* scales, float* norms) {
+    const int nb = mx4_blocks(d), ng = mx4_groups(d), lane = threadIdx.x & 31;
+    const int64_t pitch = mx4_pitch(d);
+    for (int64_t r = row0 + static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < row0 + n; r += static_cast<int64_t>(gridDim.x) * 8) {
+        const uint32_t* c = reinterpret_cast<const uint32_t*>(codes + r * pitch);
+        float nrm = 0.f;
+        for (int i = lane; i < nb * 4; i += 32) {
+            const uint32_t w = c[i];
+            float part = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 v = e2m1_values(w >> (8 * e) & 255u);
+                part = fmaf(v.x, v.x, fmaf(v.y, v.y, part));
+            }
+            const float s = e8m0_value(scales[mx4_scale_word(r, i >> 4, ng) + ((i >> 2) & 3)]);
+            nrm = fmaf(part * s, s, nrm);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) nrm += __shfl_xor_sync(0xFFFFFFFFu, nrm, o);
+        if (lane == 0) norms[r] = nrm;
+    }
+}
+
+inline unsigned warp_blocks(int64_t n) { return static_cast<unsigned>(std::min<int64_t>((n + 7) / 8, 148 * 64)); }
+
 template <typename T>
 bool rows_aligned(const void* p, int64_t ld) {   // 16-byte loads of eight elements
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0;
@@ -398,7 +456,7 @@ cudaError_t rms_rows(const RmsNormArgs& a, cudaStream_t st) {
 template <typename T>
 cudaError_t rms_type(const RmsNormArgs& a, cudaStream_t st) {
     const bool vec = rows_aligned<T>(a.x, a.ldx) && rows_aligned<T>(a.weight, 0) &&
-                     (!a.residual || (rows_aligned<T>(a.residual, a.ldr) && rows_aligned<T>(a.sum, a.lds))) &&
+                     (!a.residual || rows_aligned<T>(a.residual, a.ldr)) && (!a.sum || rows_aligned<T>(a.sum, a.lds)) &&
                      reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.ldq % 8 == 0;
     return vec ? rms_rows<T, true>(a, st) : rms_rows<T, false>(a, st);
 }
@@ -437,6 +495,23 @@ cudaError_t mx4_values(int64_t row0, int64_t n, int d, const uint8_t* codes, con
 }
 
 }  // namespace
+
+cudaError_t launch_mx4_move_scales(int d, int64_t from, int64_t to, uint8_t* scales, cudaStream_t st) {
+    mx4_move_scales_kernel<<<1, 64, 0, st>>>(mx4_groups(d), from, to, scales);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_mx4_pack_rows(int64_t n, int d, int64_t row0, uint8_t* codes, uint8_t* scales, uint8_t* plain, bool out,
+                                 cudaStream_t st) {
+    mx4_pack_rows_kernel<<<warp_blocks(n), 256, 0, st>>>(n, d, row0, codes, scales, plain, out ? 1 : 0);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_mx4_norms(int64_t n, int d, int64_t row0, const uint8_t* codes, const uint8_t* scales, float* norms,
+                             cudaStream_t st) {
+    mx4_norms_kernel<<<warp_blocks(n), 256, 0, st>>>(n, d, row0, codes, scales, norms);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_rms_norm_i8(int dtype, const RmsNormArgs& a, cudaStream_t st) {
     switch (dtype) {

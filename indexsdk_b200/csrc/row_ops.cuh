@@ -27,7 +27,7 @@ struct RmsNormArgs {
     int64_t ldx;
     const void* residual;   // or nullptr
     int64_t ldr;
-    void* sum;              // with residual
+    void* sum;              // or nullptr; with residual only
     int64_t lds;
     const void* weight;
     float eps;
@@ -46,5 +46,14 @@ cudaError_t launch_mx4_quantize(int dtype, int64_t n, int d, const void* x, int6
                                 uint8_t* scales, float* norms, cudaStream_t stream);
 cudaError_t launch_mx4_dequantize(int64_t row0, int64_t n, int d, const uint8_t* codes, const uint8_t* scales, int dtype,
                                   void* out, int64_t ldo, cudaStream_t stream);
+
+// Scales of row `from` -> row `to`.
+cudaError_t launch_mx4_move_scales(int d, int64_t from, int64_t to, uint8_t* scales, cudaStream_t stream);
+// n rows from row0 on <-> a plain array that holds each row's codes and then its nb scale bytes (out: true, into it).
+cudaError_t launch_mx4_pack_rows(int64_t n, int d, int64_t row0, uint8_t* codes, uint8_t* scales, uint8_t* plain, bool out,
+                                 cudaStream_t stream);
+// Squared norms of rows row0 .. row0 + n - 1 into the same places of norms.
+cudaError_t launch_mx4_norms(int64_t n, int d, int64_t row0, const uint8_t* codes, const uint8_t* scales, float* norms,
+                             cudaStream_t stream);
 
 }  // namespace b200

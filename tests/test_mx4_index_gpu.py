@@ -1,0 +1,243 @@
+"""Flat indexes that store microscaled 4-bit rows: search against a 64-bit statement on the rounded vectors.
+
+Rows and queries are normal values: blocks have scales of 2^-3 .. 2^0, products are multiples of 2^-8 and sums stay
+below |q| |x| < 2^13 for d <= 4096, so every fp32 sum is exact and distances and labels have to be equal."""
+import numpy as np
+import pytest
+import torch
+
+import row_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def rounded(x):
+    c, s = ref.mx4_encode(np.asarray(x, np.float64))
+    return ref.mx4_values(c, s, x.shape[1])
+
+
+def expected(b, metric, vb, vq, k, keep=None, labels=None):
+    """(D, I) by key and position; rows that are no numbers, or filtered out, do not appear."""
+    score = vq @ vb.T
+    if metric == b.METRIC_L2:
+        key = (vb * vb).sum(1)[None, :] - 2 * score
+    else:
+        key = -score
+    ok = np.isfinite(key)
+    if keep is not None:
+        ok &= keep
+    n, nq = vb.shape[0], vq.shape[0]
+    D = np.full((nq, k), np.float32(3.402823466e+38), np.float32)
+    I = np.full((nq, k), -1, np.int64)
+    labels = np.arange(n) if labels is None else labels
+    for q in range(nq):
+        order = np.argsort(np.where(ok[q], key[q], np.inf), kind="stable")[:min(k, int(ok[q].sum()))]
+        d = key[q][order] + (vq[q] * vq[q]).sum() if metric == b.METRIC_L2 else -key[q][order]
+        D[q, :len(order)], I[q, :len(order)] = d, labels[order]
+    return D, I
+
+
+def check(got, want):
+    np.testing.assert_array_equal(got[1], want[1])
+    np.testing.assert_array_equal(got[0], want[0])
+
+
+def data(seed, n, nq, d):
+    rng = np.random.default_rng(seed)
+    return rng.standard_normal((n, d)).astype(np.float32), rng.standard_normal((nq, d)).astype(np.float32)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("n, nq, d, k", [(1, 1, 16, 1), (5, 3, 32, 8), (255, 1, 48, 10), (257, 130, 128, 5), (1000, 7, 256, 100),
+                                         (20000, 1, 128, 10), (30000, 129, 64, 10), (3000, 20, 1024, 50), (700, 3, 4096, 20),
+                                         (70000, 33, 96, 1), (9000, 5, 272, 1000), (200000, 65, 128, 100)])
+def test_search(b200, n, nq, d, k, metric):
+    x, q = data(n + d, n, nq, d)
+    ix = b200.IndexFlat(d, metric, b200.MX4)
+    cut = n // 3
+    if cut:
+        ix.add(x[:cut])
+    ix.add(x[cut:])
+    assert ix.ntotal == n
+    vb = rounded(x)
+    np.testing.assert_array_equal(ix.get_base(), vb.astype(np.float32))
+    check(ix.search(q, k), expected(b200, metric, vb, rounded(q), k))
+
+
+def test_rows_and_queries_on_the_device(b200):
+    x, q = data(1, 5000, 9, 160)
+    a, c = b200.IndexFlat(160, dtype=b200.MX4), b200.IndexFlat(160, dtype=b200.MX4)
+    a.add(x)
+    xd, qd = torch.from_numpy(x).cuda(), torch.from_numpy(q).cuda()
+    D, I = torch.empty(9, 30, device="cuda"), torch.empty(9, 30, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    ids = np.arange(5000, dtype=np.int64) * 3 + 7
+    c.add_device(xd.data_ptr(), 5000, ids)
+    c.search_device(qd.data_ptr(), 9, 30, D.data_ptr(), I.data_ptr())
+    Dr, Ir = a.search(q, 30)
+    check((D.cpu().numpy(), I.cpu().numpy()), (Dr, Ir * 3 + 7))
+    np.testing.assert_array_equal(c.get_ids(), ids)
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+def test_ties_go_to_the_lower_position(b200, metric):
+    """A few distinct rows, each many times: candidate lists overflow and every query is searched again."""
+    x, q = data(2, 8, 40, 64)
+    x = np.tile(x, (5000, 1))
+    ix = b200.IndexFlat(64, metric, b200.MX4)
+    ix.add(x)
+    check(ix.search(q, 20), expected(b200, metric, rounded(x), rounded(q), 20))
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+def test_masks(b200, metric):
+    x, q = data(3, 6000, 11, 128)
+    ix = b200.IndexFlat(128, metric, b200.MX4)
+    ix.add(x)
+    rng = np.random.default_rng(0)
+    keep = rng.random((11, 6000)) < 0.3
+    keep[4] = False          # leaves nothing
+    keep[5] = False
+    keep[5, 5999] = True
+    got = ix.search_with_masks(q, 15, np.packbits(keep, axis=1, bitorder="little"))
+    check(got, expected(b200, metric, rounded(x), rounded(q), 15, keep))
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+def test_rows_that_are_no_numbers(b200, metric):
+    x, q = data(4, 300, 5, 96)
+    x[7, 3], x[299, 95], x[100] = np.nan, np.inf, -np.inf
+    q[2, 40] = np.nan
+    ix = b200.IndexFlat(96, metric, b200.MX4)
+    ix.add(x)
+    check(ix.search(q, 300), expected(b200, metric, rounded(x), rounded(q), 300))
+    vb = rounded(x)
+    np.testing.assert_array_equal(ix.get_base(), vb.astype(np.float32))
+
+
+def test_remove_reset_and_add_again(b200):
+    x, q = data(5, 1500, 6, 144)
+    ix = b200.IndexFlat(144, b200.METRIC_L2, b200.MX4)
+    ix.add(x)
+    gone = [0, 1, 130, 131, 700, 1499]
+    assert ix.remove_ids(gone + [99999]) == len(gone)
+    order = list(range(1500))
+    for p in sorted(gone, reverse=True):       # the last row takes the removed one's place
+        order[p] = order[-1]
+        order.pop()
+    vb = rounded(x[order])
+    np.testing.assert_array_equal(ix.get_base(), vb.astype(np.float32))
+    check(ix.search(q, 40), expected(b200, b200.METRIC_L2, vb, rounded(q), 40, labels=np.array(order)))
+    ix.reset()
+    D, I = ix.search(q, 2)
+    assert ix.ntotal == 0 and (I == -1).all()
+    ix.add(x[:10])
+    check(ix.search(q, 12), expected(b200, b200.METRIC_L2, rounded(x[:10]), rounded(q), 12))
+
+
+def test_save_and_load(b200, tmp_path):
+    x, q = data(6, 777, 4, 80)
+    x[5, 2] = np.nan
+    x[6] = 0
+    ix = b200.IndexFlat(80, b200.METRIC_INNER_PRODUCT, b200.MX4)
+    ix.add_with_ids(x, np.arange(777)[::-1])
+    path = str(tmp_path / "mx4.b2ix")
+    ix.save(path)
+    again = b200.load_index(path)
+    assert again.dtype == b200.MX4
+    np.testing.assert_array_equal(again.get_base().view(np.uint32), ix.get_base().view(np.uint32))
+    np.testing.assert_array_equal(again.get_ids(), ix.get_ids())
+    check(again.search(q, 33), ix.search(q, 33))
+    again.add(x[:3])
+    assert again.ntotal == 780
+
+
+def test_several_indexes_together(b200):
+    parts, q = [data(10 + i, 400 + 50 * i, 1, 64)[0] for i in range(3)], data(9, 1, 7, 64)[1]
+    ixs = []
+    base = 0
+    for p in parts:
+        ix = b200.IndexFlat(64, b200.METRIC_L2, b200.MX4)
+        ix.add_with_ids(p, base + np.arange(len(p)))
+        base += len(p)
+        ixs.append(ix)
+    check(b200.search_multi(ixs, q, 25), expected(b200, b200.METRIC_L2, rounded(np.concatenate(parts)), rounded(q), 25))
+
+
+def test_refusals(b200):
+    ix = b200.IndexFlat(64, b200.METRIC_L2, b200.MX4)
+    x = np.zeros((2, 64), np.float32)
+    ix.add(x)
+    for call in (lambda: ix.add_f16(np.zeros((1, 64), np.uint16)), lambda: ix.search_f16(np.zeros((1, 64), np.uint16), 1),
+                 lambda: b200.IndexFlat(64, b200.METRIC_L2, b200.BF16), lambda: b200.IndexFlat(50, b200.METRIC_L2, b200.MX4),
+                 lambda: b200.IndexFlat(64, b200.METRIC_INT8_COSINE, b200.MX4)):
+        with pytest.raises(b200.B200IdxError) as e:
+            call()
+        assert e.value.code == 2001
+    d = torch.zeros(2, 64, device="cuda")
+    D, I = torch.empty(2, 1, device="cuda"), torch.empty(2, 1, dtype=torch.int64, device="cuda")
+    with pytest.raises(b200.B200IdxError) as e:
+        ix.search_device_noalloc(d.data_ptr(), 2, 1, D.data_ptr(), I.data_ptr())
+    assert e.value.code == 2001 and "MX4" in e.value.msg
+
+
+# ---- hidden states into an Int8Flat index ----
+@pytest.mark.parametrize("metric, static", [(0, True), (1, True), (2, False), (2, True)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_states_into_int8flat(b200, metric, static, residual):
+    """The states calls are the operator followed by add and search."""
+    rng = np.random.default_rng(20)
+    n, nq, d, k = 3000, 17, 192, 12
+    mk = lambda r: torch.from_numpy(rng.standard_normal((r, d))).to("cuda", torch.bfloat16)  # noqa: E731
+    x, q, w = mk(n), mk(nq), mk(1).view(-1)
+    rx, rq = (mk(n), mk(nq)) if residual else (None, None)
+    s = torch.tensor([0.03], device="cuda") if static else None
+    sp = s.data_ptr() if static else 0
+    ix = b200.IndexInt8Flat(d, metric)
+    D, I = torch.empty(nq, k, device="cuda"), torch.empty(nq, k, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    ids = np.arange(n, dtype=np.int64) + 5
+    for lo, hi in ((0, 1001), (1001, n)):
+        ix.add_states_device(hi - lo, b200.BF16, x[lo:hi].data_ptr(), w.data_ptr(), 1e-5, static_scale_ptr=sp, ids=ids[lo:hi],
+                             residual_ptr=rx[lo:hi].data_ptr() if residual else 0)
+    ix.search_states_device(nq, b200.BF16, q.data_ptr(), w.data_ptr(), 1e-5, k, D.data_ptr(), I.data_ptr(),
+                            residual_ptr=rq.data_ptr() if residual else 0, static_scale_ptr=sp)
+
+    def rows(t, r):
+        out = torch.empty(t.shape, dtype=torch.int8, device="cuda")
+        sc = torch.empty(t.shape[0], device="cuda")
+        b200.rms_norm_i8_device(t.shape[0], d, b200.BF16, t.data_ptr(), w.data_ptr(), 1e-5, out.data_ptr(),
+                                residual_ptr=r.data_ptr() if residual else 0, static_scale_ptr=sp,
+                                scales_ptr=0 if static else sc.data_ptr())
+        return out.cpu().numpy()
+
+    plain = b200.IndexInt8Flat(d, metric)
+    plain.add_with_ids(rows(x, rx), ids)
+    np.testing.assert_array_equal(ix.get_base(), plain.get_base())
+    np.testing.assert_array_equal(ix.get_ids(), ids)
+    Dr, Ir = plain.search(rows(q, rq), k)
+    np.testing.assert_array_equal(I.cpu().numpy(), Ir)
+    np.testing.assert_array_equal(D.cpu().numpy(), Dr)
+
+
+def test_states_refusals(b200):
+    x = torch.zeros(4, 64, device="cuda")
+    D, I = torch.empty(4, 1, device="cuda"), torch.empty(4, 1, dtype=torch.int64, device="cuda")
+    s = torch.ones(1, device="cuda")
+    ip = b200.IndexInt8Flat(64, b200.METRIC_INNER_PRODUCT)
+    ok = dict(n=4, dtype=b200.F32, x_ptr=x.data_ptr(), weight_ptr=x.data_ptr(), eps=1e-6)
+    for bad, text in ((dict(), "static_scale"), (dict(n=0), "n must"), (dict(dtype=9), "dtype"), (dict(eps=0.0), "eps"),
+                      (dict(x_ptr=0), "Invalid x"), (dict(weight_ptr=0), "Invalid weight")):
+        a = dict(ok, **bad)
+        for call in (lambda: ip.add_states_device(**a, static_scale_ptr=s.data_ptr() if bad else 0),
+                     lambda: ip.search_states_device(**a, k=1, D_ptr=D.data_ptr(), I_ptr=I.data_ptr(),
+                                                     static_scale_ptr=s.data_ptr() if bad else 0)):
+            with pytest.raises(b200.B200IdxError) as e:
+                call()
+            assert e.value.code == 2001 and text in e.value.msg
+    with pytest.raises(b200.B200IdxError):
+        ip.search_states_device(**ok, k=0, D_ptr=D.data_ptr(), I_ptr=I.data_ptr(), static_scale_ptr=s.data_ptr())
+    lib = b200.load()
+    fl = b200.IndexFlat(64)
+    assert lib.b200idx_add_states_device(fl.handle, 4, 0, x.data_ptr(), 0, x.data_ptr(), 1e-6, s.data_ptr(), None) == 2001
+    assert ip.ntotal == 0

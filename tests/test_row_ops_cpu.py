@@ -32,7 +32,7 @@ def _rms(b200, **kw):
     (dict(dtype=3), "dtype"), (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=2.0), "eps"),
     (dict(x_ptr=0), "Invalid x"), (dict(weight_ptr=0), "Invalid weight"), (dict(q_ptr=0), "Invalid q"),
     (dict(scales_ptr=0), "exactly one"), (dict(static_scale_ptr=A), "exactly one"),
-    (dict(residual_ptr=A), "residual and sum"), (dict(sum_ptr=A), "residual and sum"),
+    (dict(sum_ptr=A), "needs a residual"),
     (dict(ldx=31), "ldx"), (dict(ldq=31), "ldq"), (dict(ldr=-1), "ldr"),
     (dict(residual_ptr=A, sum_ptr=A, ldr=40), "same stride"),
     (dict(x_ptr=A + 1), "aligned"), (dict(scales_ptr=A + 2), "aligned"),
