@@ -144,8 +144,8 @@ int b200idx_merge_topk_device_strided(int nsrc, int64_t n, int k, int descending
  *      their element type unless more is said; row strides (ld) count elements, 0 = rows without gaps.
  *      Work is queued on `stream` (a cudaStream_t of that device, NULL = its default stream), nothing is
  *      allocated or waited for, calls may overlap and may be captured into a graph.  Outputs must not
- *      overlap inputs or one another except where it is allowed below.  0 < n < 1e9, 0 < d <= 16384; rows
- *      behind n and elements behind d are neither read nor written (scales: see below).
+ *      overlap inputs or one another except where it is allowed below.  0 < n < 1e9, 0 < d <= 16384.  Rows
+ *      behind n are neither read nor written, elements behind d have no influence and stay as they are.
  *      Messages of failing calls: b200idx_last_error(NULL). ----
  *
  * Root-mean-square norm with the residual's addition, rounded to int8 rows with scales: the last step of an

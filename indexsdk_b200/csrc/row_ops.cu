@@ -4,9 +4,12 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 namespace {
+
+constexpr int64_t kSms = 148;   // shapes grids, nothing else
 
 // ---- eight consecutive elements of a row <-> fp32 ----
 template <typename T>
@@ -26,203 +29,335 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Eight elements as they lie in memory: four or eight words.
 template <typename T>
-union Pack8 {
-    uint4 v[sizeof(T) / 2];
-    T e[8];
-    __device__ Pack8() {}
+struct Row8 {
+    uint32_t w[2 * sizeof(T)];
 };
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {   // 16-byte aligned
-    Pack8<T> k;
+__device__ __forceinline__ void unpack8(const Row8<T>& k, float (&f)[8]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) k.v[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(k.w[i]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f<T>(k.e[i]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&k.w[i]));
+                f[2 * i] = v.x;
+                f[2 * i + 1] = v.y;
+            } else {   // bf16 is the upper half of an fp32
+                f[2 * i] = __uint_as_float(k.w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(k.w[i] & 0xFFFF0000u);
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void pack8(const float (&f)[8], Row8<T>& k) {   // to nearest, ties to even
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k.w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                k.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                k.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, Row8<T>& k) {   // 16-byte aligned
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        k.w[4 * i] = u.x; k.w[4 * i + 1] = u.y; k.w[4 * i + 2] = u.z; k.w[4 * i + 3] = u.w;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Row8<T>& k) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(k.w[4 * i], k.w[4 * i + 1], k.w[4 * i + 2], k.w[4 * i + 3]);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-    Pack8<T> k;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k.e[i] = from_f<T>(f[i]);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = k.v[i];
+    Row8<T> k;
+    pack8<T>(f, k);
+    store8<T>(p, k);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // ---------------------------------------------------------------------------------------
-// RMS norm -> int8.  A row belongs to NT threads (a warp or a block), which keep it in registers: one pass
-// over memory, one reduction (sum of squares and the largest |s w| together -- the norm's factor is the same
-// for the whole row, so it is not needed to find the largest element, and q = round(s w * 127 / max|s w|)
-// does not contain it at all).  Thread t owns the chunks of 8 elements t, t + NT, ... (VEC) or the elements
-// t, t + NT, ... (rows that are not 16-byte aligned; loads stay coalesced).
+// RMS norm -> int8.  A row belongs to NT threads, up to 32 lanes of a warp (short rows: a reduction over few lanes,
+// several rows a warp) or a block; they keep it in registers: one pass over memory, one reduction (sum of squares and
+// the largest |s w| together -- the norm's factor is the same for the whole row, so it is not needed to find the
+// largest element, and q = round(s w * 127 / max|s w|) does not contain it at all).  Thread t owns the
+// chunks of 8 elements t, t + NT, ... (VEC) or the elements t, t + NT, ... (rows that are not 16-byte aligned;
+// loads stay coalesced).  The next row's loads are on their way while this one is reduced and written.
 // ---------------------------------------------------------------------------------------
 template <int NT>
-__device__ __forceinline__ void reduce_row(float& sum, float& top, float (&sh)[2][NT / 32 + 1]) {
+struct RowSums {
+    float ssq[2][NT / 32 + 1], top[2][NT / 32 + 1];   // two sets in turn: one is written again only behind the other's barrier
+};
+template <int NT>
+__device__ __forceinline__ void reduce_row(float& sum, float& top, RowSums<NT>& sh, int& turn) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = (NT < 32 ? NT : 32) / 2; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     }
     if (NT > 32) {
-        const int w = threadIdx.x >> 5;
-        __syncthreads();   // (the values of the reduction before have been read)
-        if ((threadIdx.x & 31) == 0) { sh[0][w] = sum; sh[1][w] = top; }
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) { sh.ssq[turn][threadIdx.x >> 5] = sum; sh.top[turn][threadIdx.x >> 5] = top; }
         __syncthreads();
-        sum = sh[0][0];
-        top = sh[1][0];
+        sum = sh.ssq[turn][0];
+        top = sh.top[turn][0];
 #pragma unroll
         for (int i = 1; i < NT / 32; ++i) {
-            sum += sh[0][i];
-            top = fmaxf(top, sh[1][i]);
+            sum += sh.ssq[turn][i];
+            top = fmaxf(top, sh.top[turn][i]);
         }
     }
 }
 
-template <typename T, bool VEC, int NT, int J>
-__global__ void __launch_bounds__(NT == 32 ? 128 : NT) rms_norm_i8_kernel(const RmsNormArgs a) {
-    __shared__ float sh[2][NT / 32 + 1];
-    constexpr int kRows = NT == 32 ? 4 : 1;   // rows a block works on at a time
-    const int t = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const T* weight = static_cast<const T*>(a.weight);
+template <typename T, bool VEC, bool RES, int NT, int J, int FIT>
+__global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(const RmsNormArgs a) {
+    __shared__ RowSums<NT> sh;
+    int turn = 0;
+    constexpr int kRows = NT <= 32 ? 128 / NT : 1;   // rows a block works on at a time
+    constexpr bool kAhead = sizeof(T) == 2;          // (fp32: the registers of a second row cost more blocks than they hide)
+    const int t = NT <= 32 ? threadIdx.x & (NT - 1) : threadIdx.x;
     // element e of chunk j of this thread
     auto at = [&](int j, int e) { return VEC ? (t + NT * j) * 8 + e : t + NT * (8 * j + e); };
     auto whole = [&](int j) { return VEC && at(j, 8) <= a.d; };
-    auto fetch = [&](const T* p, int j, float (&f)[8]) {
+    auto fetch = [&](const void* base, int j, Row8<T>& k) {
+        const T* p = static_cast<const T*>(base);
         if (whole(j)) {
-            load8<T>(p + at(j, 0), f);
-        } else {
+            load8<T>(p + at(j, 0), k);
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = at(j, e) < a.d ? to_f<T>(p[at(j, e)]) : 0.f;
+            for (int e = 0; e < 8; ++e) k.w[e] = at(j, e) < a.d ? reinterpret_cast<const uint32_t*>(p)[at(j, e)] : 0u;
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const uint32_t lo = at(j, e) < a.d ? h[at(j, e)] : 0u, hi = at(j, e + 1) < a.d ? h[at(j, e + 1)] : 0u;
+                k.w[e / 2] = lo | hi << 16;
+            }
         }
     };
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (NT == 32 ? threadIdx.x >> 5 : 0); row < a.n;
-         row += static_cast<int64_t>(gridDim.x) * kRows) {
-        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-        float v[J][8];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    const int slot = NT <= 32 ? threadIdx.x / NT : 0;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
+    // (the lanes of a warp meet in the reductions: they leave together)
+    const int64_t first = NT < 32 ? row - slot % (NT < 32 ? 32 / NT : 1) : row;
+    Row8<T> x[J], r[RES ? J : 1], s[RES ? J : 1];
+    auto fetch_row = [&](int64_t i) {
+        const T* xp = static_cast<const T*>(a.x) + i * a.ldx;
 #pragma unroll
-        for (int j = 0; j < J; ++j) fetch(x, j, v[j]);
-        T* sum_row = static_cast<T*>(a.sum) + row * a.lds;
-        if (a.residual) {
-            const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
-            float f[J][8];
+        for (int j = 0; j < J; ++j) fetch(xp, j, x[j]);
+        if (RES) {
+            const T* rp = static_cast<const T*>(a.residual) + i * a.ldr;
 #pragma unroll
-            for (int j = 0; j < J; ++j) fetch(r, j, f[j]);
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                // The sum is rounded to the rows' type BEFORE it is normalised: what is normalised is what the
-                // model carries on, so the result is that of the two steps done one after the other.
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = to_f<T>(from_f<T>(v[j][e] + f[j][e]));
-                if (!a.sum) continue;
-                if (whole(j)) {
-                    store8<T>(sum_row + at(j, 0), v[j]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (at(j, e) < a.d) sum_row[at(j, e)] = from_f<T>(v[j][e]);
-                }
-            }
+            for (int j = 0; j < J; ++j) fetch(rp, j, r[j]);
         }
-        float ssq = 0.f, top = 0.f, pre = 1.f;
+    };
+    auto weights = [&](int j, float (&f)[8]) {
+        Row8<T> k;
+        fetch(a.weight, j, k);
+        unpack8<T>(k, f);
+    };
+    if (kAhead && row < a.n) fetch_row(row);
+    for (int64_t lead = first; lead < a.n; lead += step, row += step) {
+        const bool real = row < a.n;
+        if (!kAhead && real) fetch_row(row);
+        float ssq = 0.f, top = 0.f;
+        float v[J][8];   // s w
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            float w[8];
-            fetch(weight, j, w);
+            float f[8], w[8];
+            unpack8<T>(x[j], f);
+            if (RES) {
+                // The sum is rounded to the rows' type BEFORE it is normalised: what is normalised is what the
+                // model carries on, so the result is that of the two steps done one after the other.
+                float g[8];
+                unpack8<T>(r[j], g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] += g[e];
+                pack8<T>(f, s[j]);
+                unpack8<T>(s[j], f);
+            }
+            weights(j, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                ssq = fmaf(v[j][e], v[j][e], ssq);
-                v[j][e] *= w[e];
-                top = fmaxf(top, fabsf(v[j][e]));
+                ssq = fmaf(f[e], f[e], ssq);
+                v[j][e] = f[e] * w[e];
             }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) top = max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
         }
-        reduce_row<NT>(ssq, top, sh);
-        if (!(ssq <= 3.4e38f) || !(top <= 3.4e38f)) {
-            // The squares left the range of fp32 (or the row holds no numbers): once more with values scaled by
-            // 2^-100.  The sum may have taken x's or the residual's place; this thread wrote what it reads.
-            pre = 7.8886090522101181e-31f;
-            ssq = top = 0.f;
-            const T* again = a.sum ? sum_row : x;
-            const T* r = a.residual && !a.sum ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+        if (RES && a.sum && real) {   // (before the next row is fetched: it may take this row's place in x or the residual)
+            T* sum_row = static_cast<T*>(a.sum) + row * a.lds;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                float w[8];
-                fetch(again, j, v[j]);
-                if (r) {
-                    fetch(r, j, w);
+                if (whole(j)) {
+                    store8<T>(sum_row + at(j, 0), s[j]);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[j][e] = to_f<T>(from_f<T>(v[j][e] + w[e]));
+                    for (int e = 0; e < 8; ++e) {
+                        if (at(j, e) >= a.d) continue;
+                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(sum_row)[at(j, e)] = s[j].w[e];
+                        else reinterpret_cast<uint16_t*>(sum_row)[at(j, e)] = static_cast<uint16_t>(s[j].w[e / 2] >> (16 * (e & 1)));
+                    }
                 }
-                fetch(weight, j, w);
+            }
+        }
+        if (kAhead && row + step < a.n) fetch_row(row + step);
+        float mine = top;
+        reduce_row<NT>(ssq, top, sh, turn);
+        float pre = 1.f;   // y = v * rinv, and v holds s pre w
+        // (any row of the warp: its lanes go together; rows that need none of it come out the same)
+        const bool again = !(ssq <= 3.4e38f) || !(top <= 3.4e38f);
+        if (NT < 32 ? __any_sync(0xFFFFFFFFu, again) : again) {
+            // The squares left the range of fp32 (or the row holds no numbers): once more, scaled by 2^-100.
+            if (again) pre = 7.8886090522101181e-31f;
+            ssq = top = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                float f[8], w[8];
+                if (RES) {
+                    unpack8<T>(s[RES ? j : 0], f);
+                } else {
+                    Row8<T> k;
+                    fetch(static_cast<const T*>(a.x) + (real ? row : 0) * a.ldx, j, k);
+                    unpack8<T>(k, f);
+                }
+                weights(j, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float s = v[j][e] * pre;
-                    ssq = fmaf(s, s, ssq);
-                    v[j][e] = s * w[e];
+                    const float u = f[e] * pre;
+                    ssq = fmaf(u, u, ssq);
+                    v[j][e] = u * w[e];
                     top = fmaxf(top, fabsf(v[j][e]));
                 }
             }
-            reduce_row<NT>(ssq, top, sh);
+            mine = top;
+            reduce_row<NT>(ssq, top, sh, turn);
         }
-        const float rinv = 1.f / sqrtf(ssq / static_cast<float>(a.d) + a.eps * pre * pre);   // y = v * rinv
+        const float rinv = 1.f / sqrtf(ssq / static_cast<float>(a.d) + a.eps * pre * pre);
         const bool numbers = ssq <= 3.4e38f;   // false for NaN and infinities
-        float c, up = 1.f;   // q = round(v * up * c)
+        float c;   // q = round(v c)
         if (a.static_scale) {
-            const float s = __ldg(a.static_scale);
-            c = numbers && s > 0.f && s <= 3.4e38f ? rinv / s : 0.f;
+            const float given = __ldg(a.static_scale);
+            c = numbers && given > 0.f && given <= 3.4e38f ? rinv / given : 0.f;
+            if (mine * c > 127.f) {   // (few values: a scale is made for its rows)
+                const float most = 127.f / c;
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] = fminf(fmaxf(v[j][e], -most), most);
+            }
         } else {
-            up = top < 1e-20f ? 18446744073709551616.f : 1.f;   // keeps 127 / top in range; a power of two
-            c = numbers && top > 0.f ? 127.f / (top * up) : 0.f;
-            if (t == 0) a.scales[row] = numbers ? top * rinv / 127.f : __int_as_float(0x7fc00000);
+            if (t == 0 && real) a.scales[row] = numbers ? top * rinv / 127.f : __int_as_float(0x7fc00000);
+            if (top < 1e-20f) {   // keeps 127 / top in range
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] *= 18446744073709551616.f;
+                top *= 18446744073709551616.f;
+            }
+            c = numbers && top > 0.f ? 127.f / top : 0.f;   // (leaves nothing above 127)
         }
+        if (!real) continue;
         int8_t* q = a.q + row * a.ldq;
+        const uint32_t keep = c != 0.f ? 0xFFFFFFFFu : 0u;   // rows that are zeros, or no numbers
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            int b[8];
+            // v c + 1.5 * 2^23: the last bit of such a sum is one, so it is rounded to a whole number, whose
+            // two's complement stands in the low bits (a multiply-add instead of a conversion)
+            uint32_t b[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float u = v[j][e] * up * c;
-                b[e] = c == 0.f ? 0 : __float2int_rn(fminf(fmaxf(u, -127.f), 127.f));
-            }
+            for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(fmaf(v[j][e], c, 12582912.f));
+            uint2 o;
+            o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & keep;
+            o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410) & keep;
             if (whole(j)) {
-                uint2 o;
-                o.x = (b[0] & 255) | (b[1] & 255) << 8 | (b[2] & 255) << 16 | b[3] << 24;
-                o.y = (b[4] & 255) | (b[5] & 255) << 8 | (b[6] & 255) << 16 | b[7] << 24;
                 *reinterpret_cast<uint2*>(q + at(j, 0)) = o;
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (at(j, e) < a.d) q[at(j, e)] = static_cast<int8_t>(b[e]);
+                    if (at(j, e) < a.d) q[at(j, e)] = static_cast<int8_t>((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
             }
         }
     }
 }
 
+// Quotients by a number known to the host, of 32-bit numbers: the estimate is right or one too small.
+struct Divisor {
+    uint32_t d, m;
+    explicit Divisor(uint32_t v) : d(v), m(static_cast<uint32_t>((uint64_t(1) << 32) / v - (v == 1 ? 1 : 0))) {}
+    __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+        uint32_t q = __umulhi(x, m);
+        if (x - q * d >= d) ++q;
+        return q;
+    }
+};
+constexpr int64_t kFlat = int64_t(1) << 31;   // elements (or groups) one launch covers
+
 // ---- int8 rows -> values; a thread per 8 elements ----
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) i8_dequantize_kernel(int64_t n, int d, const int8_t* q, int64_t ldq,
+// Rows without gaps (FLAT) are one long array of outputs: a thread writes 8 of them on a 16-byte boundary,
+// whatever d is, and takes the scale of the next row where a row ends among them.
+template <typename T, bool FLAT>
+__global__ void __launch_bounds__(256) i8_dequantize_kernel(uint32_t total, Divisor by, const int8_t* q, int64_t ldq,
                                                             const float* scales, const float* static_scale, T* out,
                                                             int64_t ldo) {
-    const int per = (d + 7) / 8;   // VEC: chunks of a row;  else threads of a row, each with every per-th element
-    const int64_t total = n * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t row = i / per;
-        const int c = static_cast<int>(i - row * per);
-        const float s = __ldg(scales ? scales + row : static_scale);
-        const int8_t* p = q + row * ldq;
-        T* o = out + row * ldo;
-        if (VEC && c * 8 + 8 <= d) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p + c * 8);
-            float f[8];
+    const uint32_t step = gridDim.x * 256 * (FLAT ? 8 : 1);
+    uint32_t i = (blockIdx.x * 256 + threadIdx.x) * (FLAT ? 8 : 1);
+    if (!FLAT) {
+        for (; i < total; i += step) {
+            const uint32_t row = by.quotient(i), k = i - row * by.d;
+            const float s = __ldg(scales ? scales + row : static_scale);
+            out[row * ldo + k] = from_f<T>(static_cast<float>(q[row * ldq + k]) * s);
+        }
+        return;
+    }
+    for (; i < total; i += 2 * step) {   // two pieces at a time: their loads are on the way together
+        uint2 u[2];
+        float s[2], s2[2];
+        uint32_t first[2];   // elements that belong to the first row
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                f[e] = static_cast<float>(static_cast<int8_t>((e < 4 ? u.x : u.y) >> (8 * (e & 3)))) * s;
-            store8<T>(o + c * 8, f);
-        } else {
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t at = i + p * step;
+            if (at + 8 > total) continue;
+            const uint32_t row = by.quotient(at);
+            first[p] = by.d - (at - row * by.d);
+            u[p] = *reinterpret_cast<const uint2*>(q + at);
+            s[p] = __ldg(scales ? scales + row : static_scale);
+            s2[p] = first[p] < 8 && scales ? __ldg(scales + row + 1) : s[p];   // (d >= 8)
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int k = VEC ? c * 8 + e : c + e * per;
-                if (k < d) o[k] = from_f<T>(static_cast<float>(p[k]) * s);
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t at = i + p * step;
+            if (at + 8 <= total) {
+                float f[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    f[e] = static_cast<float>(static_cast<int8_t>((e < 4 ? u[p].x : u[p].y) >> (8 * (e & 3)))) * (e < first[p] ? s[p] : s2[p]);
+                store8<T>(out + at, f);
+            } else {
+                for (uint32_t e = at; e < total; ++e)
+                    out[e] = from_f<T>(static_cast<float>(q[e]) * __ldg(scales ? scales + by.quotient(e) : static_scale));
             }
         }
     }
@@ -259,121 +394,274 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {   // 2^(byte - 127)
     return byte == 0u ? __int_as_float(0x00400000) : __int_as_float(byte == 255u ? 0x7fc00000 : byte << 23);
 }
 
-// Rounding to MX4.  Half a warp (16 threads of 8 elements, four threads a block of 32) works on one group of
-// 128 elements, so that the four scale bytes of a group leave as one word and the codes of a group as 64
-// contiguous bytes.  A warp takes whole rows (two groups at a time), which lets it add up the squared norm of
-// the rounded row on the way where an index asks for it; `split` warps share a row where there are few rows
-// (each warp then starts at a group of its own; not with norms).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) mx4_quantize_kernel(int64_t n, int d, const T* x, int64_t ldx, int64_t row0,
-                                                           uint8_t* codes, uint8_t* scales, float* norms, int split) {
-    __shared__ float stage[VEC ? 1 : 8][2][132];
-    const int lane = threadIdx.x & 31, half = lane >> 4, t = lane & 15, warp = threadIdx.x >> 5;
-    const int nb = mx4_blocks(d), ng = mx4_groups(d);
-    const int64_t pitch = mx4_pitch(d);
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + warp; u < n * split; u += warps) {
-        const int64_t row = u / split;
-        const int part = static_cast<int>(u - row * split);
-        const T* xr = x + row * ldx;
-        uint8_t* crow = codes + (row0 + row) * pitch;
-        float nrm = 0.f;
-        for (int g0 = 2 * part; g0 < ng; g0 += 2 * split) {
-            const int g = g0 + half, k = g * 128 + t * 8;   // this thread's first element
-            float f[8];
-            if (VEC) {
-                if (k + 8 <= d) {
-                    load8<T>(xr + k, f);
-                } else {
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 32 consecutive bytes of a row that starts off a 16-byte boundary: the aligned words around them, shifted.
+// `shift` is the address modulo 16 (the same for a whole row); nothing before `p` rounded down and nothing from
+// `end` on is read.
+__device__ __forceinline__ bool load32_shifted(const char* p, uint32_t shift, const char* end, uint32_t (&k)[8]) {
+    const uint4* base = reinterpret_cast<const uint4*>(p - shift);
+    if (reinterpret_cast<const char*>(base + 3) > end) return false;
+    uint32_t w[12];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = k + e < d ? to_f<T>(xr[k + e]) : 0.f;
-                }
-            } else {
-                // coalesced loads, turned to eight consecutive elements a thread in shared memory
+    for (int i = 0; i < 3; ++i) {
+        const uint4 u = __ldg(base + i);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+    }
+    if (shift & 8) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int m = g * 128 + e * 16 + t;
-                    stage[warp][half][e * 16 + t] = m < d ? to_f<T>(xr[m]) : 0.f;
-                }
-                __syncwarp();
+        for (int i = 0; i < 10; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 4) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = stage[warp][half][t * 8 + e];
-                __syncwarp();
-            }
-            float top = 0.f;
-            bool fine = true;
+        for (int i = 0; i < 9; ++i) w[i] = w[i + 1];
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                top = fmaxf(top, fabsf(f[e]));
-                fine = fine && fabsf(f[e]) <= 3.402823466e+38f;   // (NaN compares false)
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                fine = __shfl_xor_sync(0xFFFFFFFFu, static_cast<int>(fine), o) != 0 && fine;
-            }
-            // floor(log2(top)) is the exponent field; a subnormal or zero top ends at the smallest scale anyway
-            const int field = static_cast<int>(__float_as_uint(top) >> 23) - 2;
-            const int byte = fine ? max(field, 0) : 255;
-            const float inv = fine ? __int_as_float((254 - byte) << 23) : 0.f;   // 2^(127 - byte)
-            uint32_t c = 0;
-            if (fine) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c |= e2m1_pair(f[2 * e] * inv, f[2 * e + 1] * inv) << (8 * e);
-            }
-            if (norms) {
-                float part_sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 v = e2m1_values(c >> (8 * e));
-                    part_sum = fmaf(v.x, v.x, fmaf(v.y, v.y, part_sum));   // exact: at most 288, in quarters
-                }
-                if (g * 4 + (t >> 2) < nb) {
-                    const float s = e8m0_value(byte);
-                    nrm = fmaf(part_sum * s, s, nrm);
-                }
-            }
-            if (g * 4 + (t >> 2) < nb) *reinterpret_cast<uint32_t*>(crow + static_cast<int64_t>(g) * 64 + t * 4) = c;
-            uint32_t word = static_cast<uint32_t>(g * 4 + (t >> 2) < nb ? byte : 127) << (8 * (t >> 2));
-            word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-            word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
-            if (t == 0 && g < ng) *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(row0 + row, g, ng)) = word;
+    for (int i = 0; i < 8; ++i) k[i] = __funnelshift_r(w[i], w[i + 1], (shift & 3) * 8);
+    return true;
+}
+
+// Rounding to MX4 works in pieces of 32 bytes of the input, P elements to a thread (8 fp32, 16 of 16 bits): 32 / P
+// neighbouring threads make a block of 32, 128 / P a group of 128 elements, whose four scale bytes leave as one
+// word and whose codes as 64 contiguous bytes.  With half as many elements a thread, the addresses and the
+// reductions of the 16-bit types cost more than the rounding (65 536 x 4096 bf16: 153 us instead of 110).
+template <typename T>
+constexpr int kPiece = 32 / sizeof(T);
+
+enum Mx4Load { kLoadAligned, kLoadShifted, kLoadSingle };   // rows on 16-byte boundaries; only the first one; not even that
+template <typename T, int LOAD>
+__device__ __forceinline__ void fetch_piece(const T* xr, int k, int d, const T* end, float (&f)[kPiece<T>]) {
+    constexpr int P = kPiece<T>;
+    uint32_t w[8];
+    bool got = false;
+    if (k + P <= d) {
+        if (LOAD == kLoadAligned) {
+            const uint4* p = reinterpret_cast<const uint4*>(xr + k);
+            const uint4 u = __ldg(p), v = __ldg(p + 1);
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
+            got = true;
+        } else if (LOAD == kLoadShifted) {
+            got = load32_shifted(reinterpret_cast<const char*>(xr + k), static_cast<uint32_t>(reinterpret_cast<uintptr_t>(xr)) & 15u,
+                                 reinterpret_cast<const char*>(end), w);
         }
-        if (norms) {
+    }
+    if (got) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) nrm += __shfl_xor_sync(0xFFFFFFFFu, nrm, o);
-            if (lane == 0) norms[row0 + row] = nrm;
+        for (int h = 0; h < P / 8; ++h) {
+            Row8<T> r;
+            float g[8];
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) r.w[i] = w[h * 2 * sizeof(T) + i];
+            unpack8<T>(r, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[h * 8 + e] = g[e];
         }
+    } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) f[e] = k + e < d ? to_f<T>(xr[k + e]) : 0.f;
     }
 }
 
-// MX4 -> values; a thread per 8 elements (one word of codes).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) mx4_dequantize_kernel(int64_t row0, int64_t n, int d, const uint8_t* codes,
-                                                             const uint8_t* scales, T* out, int64_t ldo) {
-    const int per = (d + 7) / 8, ng = mx4_groups(d);
-    const int64_t pitch = mx4_pitch(d), total = n * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t row = i / per;
-        const int c = static_cast<int>(i - row * per);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + (row0 + row) * pitch + c * 4);
-        const int b = c >> 2;
-        const float s = e8m0_value(__ldg(scales + mx4_scale_word(row0 + row, b >> 2, ng) + (b & 3)));
-        T* o = out + row * ldo + c * 8;
+// The block's scale byte and the thread's codes.
+template <int P>
+__device__ __forceinline__ void round_piece(const float (&f)[P], uint32_t (&c)[P / 8], uint32_t& byte) {
+    float top = fabsf(f[0]);
+#pragma unroll
+    for (int e = 1; e + 1 < P; e += 2) top = max_nan(top, fabsf(f[e]), fabsf(f[e + 1]));
+    top = max_nan(top, fabsf(f[P - 1]));
+#pragma unroll
+    for (int o = 1; o < 32 / P; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    // floor(log2(top)) is the exponent field; a subnormal or zero top ends at the smallest scale anyway.  NaN and
+    // infinities have a field of 255.
+    const int field = static_cast<int>(__float_as_uint(top) >> 23 & 255u);
+    const bool fine = field < 255;
+    byte = fine ? static_cast<uint32_t>(max(field - 2, 0)) : 255u;
+    const float inv = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte)
+#pragma unroll
+    for (int h = 0; h < P / 8; ++h) {
+        uint32_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = e2m1_pair(f[8 * h + 2 * e] * inv, f[8 * h + 2 * e + 1] * inv);
+        c[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        if (!fine) c[h] = 0u;
+    }
+}
+// The scales of a group's four blocks as a word, in every thread of the group.
+template <int P>
+__device__ __forceinline__ uint32_t scale_word(uint32_t byte, uint32_t t) {
+    uint32_t word = byte << (8 * (t / (32 / P)));
+#pragma unroll
+    for (int o = 32 / P; o < 128 / P; o <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, o);
+    return word;
+}
+template <int P>
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&c)[P / 8]) {
+    if constexpr (P == 8) *reinterpret_cast<uint32_t*>(p) = c[0];
+    else *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
+}
+
+// The groups of all rows in turn.
+template <typename T, int LOAD>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(uint32_t groups, Divisor by, int d, const T* x, int64_t ldx,
+                                                           const T* end, int64_t row0, uint8_t* codes, uint8_t* scales) {
+    constexpr int P = kPiece<T>, TG = 128 / P, PB = 256 / TG;   // threads of a group, groups of a thread block
+    const uint32_t t = threadIdx.x % TG;
+    const int nb = mx4_blocks(d);
+    const int64_t pitch = mx4_pitch(d);
+    const uint32_t step = gridDim.x * PB;
+    // (a warp stays until the last of its groups is done: they meet in the shuffles)
+    for (uint32_t u = blockIdx.x * PB + threadIdx.x / TG; u - threadIdx.x % 32 / TG < groups; u += step) {
+        const bool real = u < groups;
+        const uint32_t row = by.quotient(real ? u : 0u), g = (real ? u : 0u) - row * by.d;
+        const int k = static_cast<int>(g * 128u + t * P);   // this thread's first element
+        float f[P];
+        fetch_piece<T, LOAD>(x + row * ldx, k, d, end, f);
+        uint32_t byte, c[P / 8];
+        round_piece<P>(f, c, byte);
+        const bool here = k < nb * 32;   // the block exists
+        const uint32_t word = scale_word<P>(here ? byte : 127u, t);
+        if (!real) continue;
+        if (here) store_codes<P>(codes + (row0 + row) * pitch + k / 2, c);
+        if (t == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(row0 + row, g, by.d)) = word;
+    }
+}
+
+// The same with the squared norms of the rounded rows, for an index: a warp takes whole rows.
+template <typename T, int LOAD>
+__global__ void __launch_bounds__(256) mx4_quantize_norms_kernel(int64_t n, int d, const T* x, int64_t ldx, const T* end,
+                                                                 int64_t row0, uint8_t* codes, uint8_t* scales, float* norms) {
+    constexpr int P = kPiece<T>, TG = 128 / P;
+    const int lane = threadIdx.x & 31, t = lane % TG;
+    const int nb = mx4_blocks(d), ng = mx4_groups(d);
+    const int64_t pitch = mx4_pitch(d);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < n; row += static_cast<int64_t>(gridDim.x) * 8) {
+        const T* xr = x + row * ldx;
+        uint8_t* crow = codes + (row0 + row) * pitch;
+        float nrm = 0.f;
+        for (int g0 = 0; g0 < ng; g0 += 32 / TG) {
+            const int g = g0 + lane / TG, k = g * 128 + t * P;
+            float f[P];
+            fetch_piece<T, LOAD>(xr, k, d, end, f);
+            uint32_t byte, c[P / 8];
+            round_piece<P>(f, c, byte);
+            const bool here = k < nb * 32;
+            if (here) {
+                float part = 0.f;
+#pragma unroll
+                for (int e = 0; e < P / 2; ++e) {
+                    const float2 v = e2m1_values(c[e / 4] >> (8 * (e & 3)) & 255u);
+                    part = fmaf(v.x, v.x, fmaf(v.y, v.y, part));   // exact: at most 576, in quarters
+                }
+                const float s = e8m0_value(byte);
+                nrm = fmaf(part * s, s, nrm);
+                store_codes<P>(crow + k / 2, c);
+            }
+            const uint32_t word = scale_word<P>(here ? byte : 127u, t);
+            if (t == 0 && g < ng) *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(row0 + row, g, ng)) = word;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) nrm += __shfl_xor_sync(0xFFFFFFFFu, nrm, o);
+        if (lane == 0) norms[row0 + row] = nrm;
+    }
+}
+
+// MX4 -> values where a thread's 16 bytes of output lie in one block: d a multiple of O, rows on 16-byte boundaries.
+// Neighbouring threads write neighbouring pieces (32 bytes a thread: 65 536 x 4096 to bf16 149 us instead of 135).
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_dequantize_aligned_kernel(uint32_t pieces, Divisor by, int64_t row0, int ng, int64_t pitch,
+                                                                     const uint8_t* codes, const uint8_t* scales, T* out, int64_t ldo) {
+    constexpr int O = 16 / sizeof(T);
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < pieces; i += gridDim.x * 256) {
+        const uint32_t row = by.quotient(i), c = i - row * by.d, b = c / (32 / O);   // by.d: pieces of a row; b: block
+        const uint8_t* p = codes + (row0 + row) * pitch + c * (O / 2);
+        const uint32_t w = O == 8 ? __ldg(reinterpret_cast<const uint32_t*>(p)) : __ldg(reinterpret_cast<const uint16_t*>(p));
+        const float s = e8m0_value(__ldg(scales + mx4_scale_word(row0 + row, b >> 2, ng) + (b & 3u)));
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 v = e2m1_values(w >> (8 * e) & 255u);
+        for (int e = 0; e < O / 2; ++e) {
+            const float2 v = e2m1_values(w >> (8 * e));
             f[2 * e] = v.x * s;
             f[2 * e + 1] = v.y * s;
         }
-        if (VEC && c * 8 + 8 <= d) {
-            store8<T>(o, f);
-        } else {
+        T* o = out + row * ldo + c * O;
+        if constexpr (O == 8) store8<T>(o, f);
+        else *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+}
+
+// MX4 -> values.  FLAT as in i8_dequantize_kernel: 8 outputs on a 16-byte boundary need two words of codes, shifted,
+// and up to two scales; where a row ends among them, also the next row's first word and scale.
+__device__ __forceinline__ float mx4_value(const uint8_t* crow, const uint8_t* scales, int64_t row, uint32_t k, int ng) {
+    const uint32_t b = k >> 5, code = crow[k >> 1] >> (4 * (k & 1u)) & 15u;
+    return e2m1_values(code).x * e8m0_value(__ldg(scales + mx4_scale_word(row, b >> 2, ng) + (b & 3u)));
+}
+template <typename T, bool FLAT>
+__global__ void __launch_bounds__(256) mx4_dequantize_kernel(uint32_t total, Divisor by, int64_t row0, const uint8_t* codes,
+                                                             const uint8_t* scales, T* out, int64_t ldo) {
+    const int d = static_cast<int>(by.d), nb = mx4_blocks(d), ng = mx4_groups(d);
+    const int64_t pitch = mx4_pitch(d);
+    const uint32_t step = gridDim.x * 256 * (FLAT ? 8 : 1);
+    uint32_t i = (blockIdx.x * 256 + threadIdx.x) * (FLAT ? 8 : 1);
+    if (!FLAT) {
+        for (; i < total; i += step) {
+            const uint32_t row = by.quotient(i), k = i - row * by.d;
+            out[row * ldo + k] = from_f<T>(mx4_value(codes + (row0 + row) * pitch, scales, row0 + row, k, ng));
+        }
+        return;
+    }
+    for (; i < total; i += 2 * step) {   // two pieces at a time: their loads are on the way together
+        uint32_t w0[2], w1[2], w2[2], k[2];
+        uint32_t s0[2], s1[2], s2[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c * 8 + e < d) o[e] = from_f<T>(f[e]);
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t at = i + p * step;
+            if (at + 8 > total) continue;
+            const uint32_t r = by.quotient(at);
+            const int64_t row = row0 + r;
+            k[p] = at - r * by.d;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + row * pitch) + (k[p] >> 3);
+            const bool ends = k[p] + 8 > by.d;   // (d >= 8)
+            const uint32_t b = k[p] >> 5, b2 = min((k[p] + 7) >> 5, static_cast<uint32_t>(nb - 1));
+            w0[p] = __ldg(w);
+            w1[p] = (k[p] & 7u) && (k[p] >> 3) + 1 < 4u * nb ? __ldg(w + 1) : 0u;
+            w2[p] = ends ? __ldg(reinterpret_cast<const uint32_t*>(codes + (row + 1) * pitch)) : 0u;
+            s0[p] = __ldg(scales + mx4_scale_word(row, b >> 2, ng) + (b & 3u));
+            s1[p] = b2 == b ? s0[p] : __ldg(scales + mx4_scale_word(row, b2 >> 2, ng) + (b2 & 3u));
+            s2[p] = ends ? __ldg(scales + mx4_scale_word(row + 1, 0, ng)) : 0u;
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t at = i + p * step;
+            if (at + 8 <= total) {
+                const uint32_t rest = by.d - k[p];   // elements up to the row's end
+                uint32_t c = __funnelshift_r(w0[p], w1[p], 4 * (k[p] & 7u));
+                if (rest < 8) c = (c & ((1u << (4 * rest)) - 1u)) | w2[p] << (4 * rest);
+                const uint32_t first = 32u - (k[p] & 31u);   // elements of the first block
+                const float f0 = e8m0_value(s0[p]), f1 = e8m0_value(s1[p]), f2 = e8m0_value(s2[p]);
+                float f[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e += 2) {
+                    const float2 v = e2m1_values(c >> (4 * e) & 255u);
+                    f[e] = v.x * (e >= rest ? f2 : (e < first ? f0 : f1));
+                    f[e + 1] = v.y * (e + 1 >= rest ? f2 : (e + 1 < first ? f0 : f1));
+                }
+                store8<T>(out + at, f);
+            } else {
+                for (uint32_t e = at; e < total; ++e) {
+                    const uint32_t r = by.quotient(e);
+                    out[e] = from_f<T>(mx4_value(codes + (row0 + r) * pitch, scales, row0 + r, e - r * by.d, ng));
+                }
+            }
         }
     }
 }
@@ -434,64 +722,119 @@ bool rows_aligned(const void* p, int64_t ld) {   // 16-byte loads of eight eleme
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool RES, int NT, int J, int FIT = 1>
+cudaError_t rms_launch(const RmsNormArgs& a, cudaStream_t st) {
+    const int threads = NT <= 32 ? 128 : NT, rows = NT <= 32 ? 128 / NT : 1;
+    auto kern = rms_norm_i8_kernel<T, VEC, RES, NT, J, FIT>;
+    // as many blocks as fit at a time: a row is on its way while its predecessor is worked on
+    int fit = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, 0);
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = std::min<int64_t>((a.n + rows - 1) / rows, kSms * std::max(fit, 1));
+    kern<<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+template <typename T, bool VEC, bool RES>
 cudaError_t rms_rows(const RmsNormArgs& a, cudaStream_t st) {
-    const int64_t most = 148 * 64;
-    auto go = [&](auto nt, auto j) {
-        constexpr int NT = decltype(nt)::value, J = decltype(j)::value;
-        constexpr int kRows = NT == 32 ? 4 : 1;
-        const int64_t blocks = std::min<int64_t>((a.n + kRows - 1) / kRows, most);
-        rms_norm_i8_kernel<T, VEC, NT, J><<<static_cast<unsigned>(blocks), NT == 32 ? 128 : NT, 0, st>>>(a);
-        return cudaGetLastError();
-    };
-    using std::integral_constant;
-    if (a.d <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    if (a.d <= 512) return go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
-    if (a.d <= 1024) return go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-    if (a.d <= 2048) return go(integral_constant<int, 128>{}, integral_constant<int, 2>{});
-    if (a.d <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    if (a.d <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-    return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+    // 32 or 48 bytes of x a thread
+    if constexpr (sizeof(T) == 2) {
+        if (a.d <= 128) return rms_launch<T, VEC, RES, 8, 2, 6>(a, st);
+        if (a.d <= 256) return rms_launch<T, VEC, RES, 16, 2, 6>(a, st);
+        if (a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 6>(a, st);
+        if (a.d <= 768) return rms_launch<T, VEC, RES, 32, 3, 4>(a, st);
+        if (a.d <= 1024) return rms_launch<T, VEC, RES, 64, 2, 12>(a, st);
+        if (a.d <= 2048) return rms_launch<T, VEC, RES, 128, 2, 6>(a, st);
+        if (a.d <= 4096) return rms_launch<T, VEC, RES, 256, 2, 3>(a, st);
+        if (a.d <= 8192) return rms_launch<T, VEC, RES, 512, 2, 2>(a, st);
+        return rms_launch<T, VEC, RES, 512, 4>(a, st);
+    } else {
+        if (a.d <= 128) return rms_launch<T, VEC, RES, 16, 1, 8>(a, st);
+        if (a.d <= 256) return rms_launch<T, VEC, RES, 32, 1, 8>(a, st);
+        if (a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 6>(a, st);
+        if (a.d <= 1024) return rms_launch<T, VEC, RES, 64, 2, 12>(a, st);
+        if (a.d <= 2048) return rms_launch<T, VEC, RES, 128, 2, 6>(a, st);
+        if (a.d <= 4096) return rms_launch<T, VEC, RES, 256, 2, 4>(a, st);
+        if (a.d <= 8192) return rms_launch<T, VEC, RES, 512, 2, 2>(a, st);
+        return rms_launch<T, VEC, RES, 512, 4>(a, st);
+    }
 }
 template <typename T>
 cudaError_t rms_type(const RmsNormArgs& a, cudaStream_t st) {
     const bool vec = rows_aligned<T>(a.x, a.ldx) && rows_aligned<T>(a.weight, 0) &&
                      (!a.residual || rows_aligned<T>(a.residual, a.ldr)) && (!a.sum || rows_aligned<T>(a.sum, a.lds)) &&
                      reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && a.ldq % 8 == 0;
-    return vec ? rms_rows<T, true>(a, st) : rms_rows<T, false>(a, st);
+    if (a.residual) return vec ? rms_rows<T, true, true>(a, st) : rms_rows<T, false, true>(a, st);
+    return vec ? rms_rows<T, true, false>(a, st) : rms_rows<T, false, false>(a, st);
 }
 
-inline unsigned chunk_blocks(int64_t n, int d) {   // a thread per 8 elements
-    const int64_t b = (n * ((d + 7) / 8) + 255) / 256;
-    return static_cast<unsigned>(std::min<int64_t>(b, 148 * 256));
+// A launch per stretch of rows whose elements 32 bits count; a stretch is a multiple of 8 rows, which keeps
+// the 16-byte boundaries of rows without gaps.
+template <typename F>
+cudaError_t by_stretches(int64_t n, int64_t per_row, F&& go) {
+    const int64_t most = kFlat / per_row / 8 * 8;
+    for (int64_t r = 0; r < n; r += most) {
+        const cudaError_t e = go(r, std::min(most, n - r));
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
+inline unsigned flat_blocks(int64_t threads) { return static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, kSms * 64)); }
+
 template <typename T>
 cudaError_t i8_values(int64_t n, int d, const int8_t* q, int64_t ldq, const float* scales, const float* one, void* out,
                       int64_t ldo, cudaStream_t st) {
-    const bool vec = rows_aligned<T>(out, ldo) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
-    if (vec) i8_dequantize_kernel<T, true><<<chunk_blocks(n, d), 256, 0, st>>>(n, d, q, ldq, scales, one, static_cast<T*>(out), ldo);
-    else i8_dequantize_kernel<T, false><<<chunk_blocks(n, d), 256, 0, st>>>(n, d, q, ldq, scales, one, static_cast<T*>(out), ldo);
-    return cudaGetLastError();
+    const bool flat = ldo == d && ldq == d && d >= 8 && rows_aligned<T>(out, 0) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+    return by_stretches(n, d, [&](int64_t r, int64_t m) {
+        const int8_t* qr = q + r * ldq;
+        const float* sr = scales ? scales + r : nullptr;
+        T* o = static_cast<T*>(out) + r * ldo;
+        const uint32_t total = static_cast<uint32_t>(m * d);
+        if (flat) i8_dequantize_kernel<T, true><<<flat_blocks((total + 7) / 8), 256, 0, st>>>(total, Divisor(d), qr, ldq, sr, one, o, ldo);
+        else i8_dequantize_kernel<T, false><<<flat_blocks(total), 256, 0, st>>>(total, Divisor(d), qr, ldq, sr, one, o, ldo);
+        return cudaGetLastError();
+    });
+}
+template <typename T, int LOAD>
+cudaError_t mx4_round_rows(int64_t n, int d, const T* x, int64_t ldx, int64_t row0, uint8_t* codes, uint8_t* scales,
+                           float* norms, cudaStream_t st) {
+    const T* end = x + (n - 1) * ldx + d;
+    if (norms) {
+        mx4_quantize_norms_kernel<T, LOAD><<<warp_blocks(n), 256, 0, st>>>(n, d, x, ldx, end, row0, codes, scales, norms);
+        return cudaGetLastError();
+    }
+    const int ng = mx4_groups(d);
+    return by_stretches(n, ng, [&](int64_t r, int64_t m) {
+        const uint32_t groups = static_cast<uint32_t>(m * ng);
+        mx4_quantize_kernel<T, LOAD><<<flat_blocks(int64_t(groups) * (128 / kPiece<T>)), 256, 0, st>>>(groups, Divisor(ng), d, x + r * ldx, ldx, end, row0 + r, codes, scales);
+        return cudaGetLastError();
+    });
 }
 template <typename T>
 cudaError_t mx4_round(int64_t n, int d, const void* x, int64_t ldx, int64_t row0, uint8_t* codes, uint8_t* scales,
                       float* norms, cudaStream_t st) {
-    const int pairs = (mx4_groups(d) + 1) / 2;
-    int split = 1;
-    if (!norms)   // few long rows: a warp for every two groups
-        while (split < pairs && n * split < 148 * 8) ++split;
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n * split + 7) / 8, 148 * 64));
     const T* xt = static_cast<const T*>(x);
-    if (rows_aligned<T>(x, ldx)) mx4_quantize_kernel<T, true><<<blocks, 256, 0, st>>>(n, d, xt, ldx, row0, codes, scales, norms, split);
-    else mx4_quantize_kernel<T, false><<<blocks, 256, 0, st>>>(n, d, xt, ldx, row0, codes, scales, norms, split);
-    return cudaGetLastError();
+    if (rows_aligned<T>(x, ldx)) return mx4_round_rows<T, kLoadAligned>(n, d, xt, ldx, row0, codes, scales, norms, st);
+    if (rows_aligned<T>(x, 0)) return mx4_round_rows<T, kLoadShifted>(n, d, xt, ldx, row0, codes, scales, norms, st);
+    return mx4_round_rows<T, kLoadSingle>(n, d, xt, ldx, row0, codes, scales, norms, st);
 }
 template <typename T>
 cudaError_t mx4_values(int64_t row0, int64_t n, int d, const uint8_t* codes, const uint8_t* scales, void* out,
                        int64_t ldo, cudaStream_t st) {
-    if (rows_aligned<T>(out, ldo)) mx4_dequantize_kernel<T, true><<<chunk_blocks(n, d), 256, 0, st>>>(row0, n, d, codes, scales, static_cast<T*>(out), ldo);
-    else mx4_dequantize_kernel<T, false><<<chunk_blocks(n, d), 256, 0, st>>>(row0, n, d, codes, scales, static_cast<T*>(out), ldo);
-    return cudaGetLastError();
+    constexpr int O = 16 / sizeof(T);
+    if (d % O == 0 && rows_aligned<T>(out, ldo))
+        return by_stretches(n, d, [&](int64_t r, int64_t m) {
+            const uint32_t pieces = static_cast<uint32_t>(m * (d / O));
+            mx4_dequantize_aligned_kernel<T><<<flat_blocks(pieces), 256, 0, st>>>(pieces, Divisor(d / O), row0 + r, mx4_groups(d), mx4_pitch(d), codes, scales, static_cast<T*>(out) + r * ldo, ldo);
+            return cudaGetLastError();
+        });
+    const bool flat = ldo == d && d >= 8 && rows_aligned<T>(out, 0);
+    return by_stretches(n, d, [&](int64_t r, int64_t m) {
+        T* o = static_cast<T*>(out) + r * ldo;
+        const uint32_t total = static_cast<uint32_t>(m * d);
+        if (flat) mx4_dequantize_kernel<T, true><<<flat_blocks((total + 7) / 8), 256, 0, st>>>(total, Divisor(d), row0 + r, codes, scales, o, ldo);
+        else mx4_dequantize_kernel<T, false><<<flat_blocks(total), 256, 0, st>>>(total, Divisor(d), row0 + r, codes, scales, o, ldo);
+        return cudaGetLastError();
+    });
 }
 
 }  // namespace
