@@ -105,37 +105,97 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // largest element, and q = round(s w * 127 / max|s w|) does not contain it at all).  Thread t owns the
 // chunks of 8 elements t, t + NT, ... (VEC) or the elements t, t + NT, ... (rows that are not 16-byte aligned;
 // loads stay coalesced).  The next row's loads are on their way while this one is reduced and written.
+//
+// A rounding to whole numbers shows every error of its argument where that lies next to a border, and for 16-bit
+// rows with weights of 16 bits one element in 20 000 lies exactly ON a border.  So squares are added up in fp32 over
+// eight elements only, fp32 rows keep what the largest product loses to its rounding, and an element whose fp32
+// quotient is within 2^-14 of a border (that quotient is off by at most 127 * 6 * 2^-24) is compared with it in 64 bits.
 // ---------------------------------------------------------------------------------------
 template <int NT>
-struct RowSums {
-    float ssq[2][NT / 32 + 1], top[2][NT / 32 + 1];   // two sets in turn: one is written again only behind the other's barrier
+struct RowSums {   // two sets in turn: one is written again only behind the other's barrier
+    double ssq[2][NT / 32 + 1], top[2][NT / 32 + 1];
 };
-template <int NT>
-__device__ __forceinline__ void reduce_row(float& sum, float& top, RowSums<NT>& sh, int& turn) {
+// The sum of `sum` and the largest `top` of the row's threads.
+template <int NT, typename F>
+__device__ __forceinline__ void reduce_row(double& sum, F& top, RowSums<NT>& sh, int& turn) {
 #pragma unroll
     for (int o = (NT < 32 ? NT : 32) / 2; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const F other = __shfl_xor_sync(0xFFFFFFFFu, top, o);
+        top = other > top ? other : top;
     }
     if (NT > 32) {
         turn ^= 1;
-        if ((threadIdx.x & 31) == 0) { sh.ssq[turn][threadIdx.x >> 5] = sum; sh.top[turn][threadIdx.x >> 5] = top; }
+        if ((threadIdx.x & 31) == 0) {
+            sh.ssq[turn][threadIdx.x >> 5] = sum;
+            *reinterpret_cast<F*>(&sh.top[turn][threadIdx.x >> 5]) = top;
+        }
         __syncthreads();
         sum = sh.ssq[turn][0];
-        top = sh.top[turn][0];
+        top = *reinterpret_cast<const F*>(&sh.top[turn][0]);
 #pragma unroll
         for (int i = 1; i < NT / 32; ++i) {
             sum += sh.ssq[turn][i];
-            top = fmaxf(top, sh.top[turn][i]);
+            const F other = *reinterpret_cast<const F*>(&sh.top[turn][i]);
+            top = other > top ? other : top;
         }
     }
 }
 
+// What is rare, element by element from memory and in 64 bits.
+template <typename T, bool RES>
+__device__ __forceinline__ double row_element(const RmsNormArgs& a, int64_t row, int k) {
+    if (!RES) return to_f<T>(static_cast<const T*>(a.x)[row * a.ldx + k]);
+    if (a.sum) return to_f<T>(static_cast<const T*>(a.sum)[row * a.lds + k]);   // (this thread's own; it may have x's place)
+    return to_f<T>(from_f<T>(to_f<T>(static_cast<const T*>(a.x)[row * a.ldx + k]) +
+                             to_f<T>(static_cast<const T*>(a.residual)[row * a.ldr + k])));
+}
+// One element: its product times num / den.
+template <typename T, bool RES>
+__device__ __noinline__ void round_precisely(const RmsNormArgs& a, int64_t row, int k, double num, double den) {
+    const double y = row_element<T, RES>(a, row, k) * to_f<T>(static_cast<const T*>(a.weight)[k]) * num / den;
+    a.q[row * a.ldq + k] = static_cast<int8_t>(__double2int_rn(fmin(fmax(y, -127.), 127.)));
+}
+// A whole row: squares or products outside the range of fp32, or no numbers at all.  Every thread of the row.
+template <typename T, bool VEC, bool RES, int NT, int J>
+__device__ __noinline__ int hard_row(const RmsNormArgs& a, int64_t row, int t, bool mine, RowSums<NT>& sh, int turn) {
+    double ssq = 0., top = 0.;
+    for (int i = 0; i < 8 * J; ++i) {
+        const int k = VEC ? (t + NT * (i >> 3)) * 8 + (i & 7) : t + NT * i;
+        if (!mine || k >= a.d) continue;
+        const double s = row_element<T, RES>(a, row, k);
+        ssq += s * s;
+        top = fmax(top, fabs(s * to_f<T>(static_cast<const T*>(a.weight)[k])));
+    }
+    reduce_row<NT>(ssq, top, sh, turn);
+    if (!mine) return turn;
+    const double inf = __longlong_as_double(0x7ff0000000000000ll);
+    bool live = ssq < inf && top < inf;   // false for NaN and infinities
+    const double root = sqrt(ssq / a.d + static_cast<double>(a.eps));
+    if (!a.static_scale && t == 0) a.scales[row] = live ? static_cast<float>(top / (127. * root)) : __int_as_float(0x7fc00000);
+    double num = 127., den = top;
+    if (a.static_scale) {
+        const float given = __ldg(a.static_scale);
+        live = live && given > 0.f && given <= 3.4e38f;
+        num = 1.;
+        den = root * given;
+    }
+    live = live && den > 0.;
+    for (int i = 0; i < 8 * J; ++i) {
+        const int k = VEC ? (t + NT * (i >> 3)) * 8 + (i & 7) : t + NT * i;
+        if (k >= a.d) continue;
+        if (live) round_precisely<T, RES>(a, row, k, num, den);
+        else a.q[row * a.ldq + k] = 0;
+    }
+    return turn;
+}
+
 template <typename T, bool VEC, bool RES, int NT, int J, int FIT>
-__global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(const RmsNormArgs a) {
+__global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(const __grid_constant__ RmsNormArgs a) {
     __shared__ RowSums<NT> sh;
     int turn = 0;
     constexpr int kRows = NT <= 32 ? 128 / NT : 1;   // rows a block works on at a time
+    constexpr bool kLow = sizeof(T) == 4;            // (products of 16-bit numbers are exact in fp32)
     constexpr bool kAhead = sizeof(T) == 2;          // (fp32: the registers of a second row cost more blocks than they hide)
     const int t = NT <= 32 ? threadIdx.x & (NT - 1) : threadIdx.x;
     // element e of chunk j of this thread
@@ -162,7 +222,7 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
     int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
     // (the lanes of a warp meet in the reductions: they leave together)
     const int64_t first = NT < 32 ? row - slot % (NT < 32 ? 32 / NT : 1) : row;
-    Row8<T> x[J], r[RES ? J : 1], s[RES ? J : 1];
+    Row8<T> x[J], r[RES ? J : 1];
     auto fetch_row = [&](int64_t i) {
         const T* xp = static_cast<const T*>(a.x) + i * a.ldx;
 #pragma unroll
@@ -173,16 +233,12 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             for (int j = 0; j < J; ++j) fetch(rp, j, r[j]);
         }
     };
-    auto weights = [&](int j, float (&f)[8]) {
-        Row8<T> k;
-        fetch(a.weight, j, k);
-        unpack8<T>(k, f);
-    };
     if (kAhead && row < a.n) fetch_row(row);
     for (int64_t lead = first; lead < a.n; lead += step, row += step) {
         const bool real = row < a.n;
         if (!kAhead && real) fetch_row(row);
-        float ssq = 0.f, top = 0.f;
+        double ssq = 0.;
+        float top = 0.f, top_s = 0.f, top_w = 0.f;
         float v[J][8];   // s w
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -195,100 +251,95 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
                 unpack8<T>(r[j], g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] += g[e];
-                pack8<T>(f, s[j]);
-                unpack8<T>(s[j], f);
-            }
-            weights(j, w);
+                Row8<T> s;
+                pack8<T>(f, s);
+                unpack8<T>(s, f);
+                // (written before the next row is fetched, which may have x's or the residual's place)
+                if (a.sum && real) {
+                    T* sum_row = static_cast<T*>(a.sum) + row * a.lds;
+                    if (whole(j)) {
+                        store8<T>(sum_row + at(j, 0), s);
+                    } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ssq = fmaf(f[e], f[e], ssq);
-                v[j][e] = f[e] * w[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) top = max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
-        }
-        if (RES && a.sum && real) {   // (before the next row is fetched: it may take this row's place in x or the residual)
-            T* sum_row = static_cast<T*>(a.sum) + row * a.lds;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                if (whole(j)) {
-                    store8<T>(sum_row + at(j, 0), s[j]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (at(j, e) >= a.d) continue;
-                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(sum_row)[at(j, e)] = s[j].w[e];
-                        else reinterpret_cast<uint16_t*>(sum_row)[at(j, e)] = static_cast<uint16_t>(s[j].w[e / 2] >> (16 * (e & 1)));
+                        for (int e = 0; e < 8; ++e) {
+                            if (at(j, e) >= a.d) continue;
+                            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(sum_row)[at(j, e)] = s.w[e];
+                            else reinterpret_cast<uint16_t*>(sum_row)[at(j, e)] = static_cast<uint16_t>(s.w[e / 2] >> (16 * (e & 1)));
+                        }
                     }
                 }
             }
+            Row8<T> wt;
+            fetch(a.weight, j, wt);
+            unpack8<T>(wt, w);
+            float part = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                part = fmaf(f[e], f[e], part);
+                v[j][e] = f[e] * w[e];
+                if (kLow && fabsf(v[j][e]) > top) {
+                    top = fabsf(v[j][e]);
+                    top_s = f[e];
+                    top_w = w[e];
+                }
+            }
+            ssq += part;
+            if (!kLow) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) top = max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
+            }
         }
         if (kAhead && row + step < a.n) fetch_row(row + step);
-        float mine = top;
-        reduce_row<NT>(ssq, top, sh, turn);
-        float pre = 1.f;   // y = v * rinv, and v holds s pre w
-        // (any row of the warp: its lanes go together; rows that need none of it come out the same)
-        const bool again = !(ssq <= 3.4e38f) || !(top <= 3.4e38f);
-        if (NT < 32 ? __any_sync(0xFFFFFFFFu, again) : again) {
-            // The squares left the range of fp32 (or the row holds no numbers): once more, scaled by 2^-100.
-            if (again) pre = 7.8886090522101181e-31f;
-            ssq = top = 0.f;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                float f[8], w[8];
-                if (RES) {
-                    unpack8<T>(s[RES ? j : 0], f);
-                } else {
-                    Row8<T> k;
-                    fetch(static_cast<const T*>(a.x) + (real ? row : 0) * a.ldx, j, k);
-                    unpack8<T>(k, f);
-                }
-                weights(j, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = f[e] * pre;
-                    ssq = fmaf(u, u, ssq);
-                    v[j][e] = u * w[e];
-                    top = fmaxf(top, fabsf(v[j][e]));
-                }
-            }
-            mine = top;
+        const float mine = top;
+        double most = 0.;   // the largest product
+        if (kLow) {
+            most = fabs(static_cast<double>(top_s) * top_w);
+            reduce_row<NT>(ssq, most, sh, turn);
+            top = static_cast<float>(most);
+        } else {
             reduce_row<NT>(ssq, top, sh, turn);
+            most = top;
         }
-        const float rinv = 1.f / sqrtf(ssq / static_cast<float>(a.d) + a.eps * pre * pre);
-        const bool numbers = ssq <= 3.4e38f;   // false for NaN and infinities
-        float c;   // q = round(v c)
+        const bool hard = !(ssq <= 3e38) || !(top <= 1e36f) || (top < 1e-20f && top > 0.f);
+        if (NT < 32 ? __any_sync(0xFFFFFFFFu, hard) : hard) {
+            turn = hard_row<T, VEC, RES, NT, J>(a, row, t, hard && real, sh, turn);
+            if (hard) continue;
+        }
+        // (a warp's rows that were not hard go on)
+        const float root = sqrtf(static_cast<float>(ssq) / a.d + a.eps);   // y = v / root
+        float c = 0.f;   // q = round(v c); 0: zeros
         if (a.static_scale) {
             const float given = __ldg(a.static_scale);
-            c = numbers && given > 0.f && given <= 3.4e38f ? rinv / given : 0.f;
+            if (given > 0.f && given <= 3.4e38f) c = fminf(1.f / root / given, 3e38f);
             if (mine * c > 127.f) {   // (few values: a scale is made for its rows)
-                const float most = 127.f / c;
+                const float cut = 127.f / c;
 #pragma unroll
                 for (int j = 0; j < J; ++j)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[j][e] = fminf(fmaxf(v[j][e], -most), most);
+                    for (int e = 0; e < 8; ++e) v[j][e] = fminf(fmaxf(v[j][e], -cut), cut);
             }
         } else {
-            if (t == 0 && real) a.scales[row] = numbers ? top * rinv / 127.f : __int_as_float(0x7fc00000);
-            if (top < 1e-20f) {   // keeps 127 / top in range
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[j][e] *= 18446744073709551616.f;
-                top *= 18446744073709551616.f;
-            }
-            c = numbers && top > 0.f ? 127.f / top : 0.f;   // (leaves nothing above 127)
+            if (t == 0 && real) a.scales[row] = top / root / 127.f;
+            if (top > 0.f) c = 127.f / top;
         }
         if (!real) continue;
         int8_t* q = a.q + row * a.ldq;
-        const uint32_t keep = c != 0.f ? 0xFFFFFFFFu : 0u;   // rows that are zeros, or no numbers
+        const uint32_t keep = c != 0.f ? 0xFFFFFFFFu : 0u;   // rows that are zeros
+        uint32_t near = 0;   // chunks with an element next to a border
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            // v c + 1.5 * 2^23: the last bit of such a sum is one, so it is rounded to a whole number, whose
-            // two's complement stands in the low bits (a multiply-add instead of a conversion)
+            // v c + 1.5 * 2^23: the last bit of such a sum is one, so it is rounded to a whole number, whose two's
+            // complement stands in the low bits (a multiply-add instead of a conversion)
             uint32_t b[8];
+            float off = 0.f;   // largest distance to the whole number
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(fmaf(v[j][e], c, 12582912.f));
+            for (int e = 0; e < 8; e += 2) {
+                const float r0 = fmaf(v[j][e], c, 12582912.f), r1 = fmaf(v[j][e + 1], c, 12582912.f);
+                b[e] = __float_as_uint(r0);
+                b[e + 1] = __float_as_uint(r1);
+                off = max3(off, fabsf(fmaf(v[j][e], c, 12582912.f - r0)), fabsf(fmaf(v[j][e + 1], c, 12582912.f - r1)));
+            }
+            if (off > 0.5f - 1.f / 16384.f) near |= 1u << j;
             uint2 o;
             o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & keep;
             o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410) & keep;
@@ -298,6 +349,29 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (at(j, e) < a.d) q[at(j, e)] = static_cast<int8_t>((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
+            }
+        }
+        if (near & keep) {
+            double num = 127., den = most;
+            if (a.static_scale) {
+                num = 1.;
+                den = sqrt(ssq / a.d + static_cast<double>(a.eps)) * __ldg(a.static_scale);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                if (!(near >> j & 1u)) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float p = fabsf(v[j][e] * c), k = floorf(p);
+                    if (fabsf(p - k - 0.5f) > 1.f / 8192.f || at(j, e) >= a.d) continue;
+                    // |product| num / den against k + 1/2, without a division
+                    const double product = kLow ? row_element<T, RES>(a, row, at(j, e)) * to_f<T>(static_cast<const T*>(a.weight)[at(j, e)])
+                                                : static_cast<double>(v[j][e]);
+                    const double l = fabs(product) * num, h = (k + 0.5) * den;
+                    const int up = l > h || (l == h && (static_cast<int>(k) & 1)) ? 1 : 0;
+                    const int whole_number = static_cast<int>(k) + up;
+                    q[at(j, e)] = static_cast<int8_t>(v[j][e] < 0.f ? -whole_number : whole_number);
+                }
             }
         }
     }
