@@ -1,6 +1,7 @@
-// Products of microscaled 4-bit rows with tcgen05.mma kind::mxf4 (E2M1 codes, a scale per 32 elements).
+// Distances of microscaled 4-bit rows with tcgen05.mma kind::mxf4 (E2M1 codes, a scale per 32 elements) and the
+// selection in the epilogue.
 //
-// A CTA computes 128 x 256 tiles (rows of a x rows of b) of fp32 accumulators in TMEM:
+// A CTA computes 128 x 256 tiles (queries x base rows) of fp32 accumulators in TMEM:
 //   warp 0 (one lane)  : producer.  Per K chunk of 128 bytes (256 elements) two tensor copies (128 and 256 rows,
 //                        SWIZZLE_128B) and up to three copies of scales into a ring of four 51 KB stages.  The
 //                        scales lie in memory in the order the tensor core wants, 512 bytes for 128 rows x 4
@@ -13,9 +14,6 @@
 // accumulators therefore SHARE 96 columns (0-255 and 160-415; scales 416-511): tile t + 1 may start once tile t's
 // shared columns are in registers, which half of the epilogue warps report.
 #include "mx4_gemm.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cstring>
@@ -37,59 +35,13 @@ constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kAcc1 = 160, kScaleCols = 416, kScaleSlot = 24;   // TMEM columns
-constexpr int kModeDense = 2;
 
 struct Mx4Args {
     GemmArgs g;
     const uint8_t* a_scales;
     const uint8_t* b_scales;
     int nb, ng;      // blocks of a row, groups of four
-    // kModeDense
-    void* out;
-    int64_t ldo;
-    int dtype;
-    int vec;         // rows of out start on 16-byte boundaries
 };
-
-// 32 accumulator columns of one row -> out[0 .. nvalid)
-template <typename T>
-__device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], T* o, int nvalid, bool vec) {
-    constexpr int kPer = 16 / sizeof(T);
-    if (vec && nvalid >= 32) {
-#pragma unroll
-        for (int i = 0; i < 32 / kPer; ++i) {
-            uint4 u;
-            if constexpr (sizeof(T) == 4) {
-                u = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-            } else {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float lo = __uint_as_float(r[8 * i + 2 * j]), hi = __uint_as_float(r[8 * i + 2 * j + 1]);
-                    if constexpr (std::is_same<T, __half>::value) {
-                        const __half2 h = __floats2half2_rn(lo, hi);
-                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                    } else {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                    }
-                }
-                u = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            reinterpret_cast<uint4*>(o)[i] = u;
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-            if (c < nvalid) {
-                const float v = __uint_as_float(r[c]);
-                if constexpr (std::is_same<T, float>::value) o[c] = v;
-                else if constexpr (std::is_same<T, __half>::value) o[c] = __float2half_rn(v);
-                else o[c] = __float2bfloat16_rn(v);
-            }
-        }
-    }
-}
 
 template <int MODE, int BURST, bool L2>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -198,9 +150,8 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
     } else {
         const int quarter = warp & 3, part = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
         const uint32_t* gnorm = static_cast<const uint32_t*>(a.bnorm);
-        RowEpilogue<float, MODE == kModeDense ? kModeAppend : MODE, BURST, false, 2, false, !L2> epi(a);
+        RowEpilogue<float, MODE, BURST, false, 2, false, !L2> epi(a);
         uint32_t t = 0;
-        bool ok = true;
         ItemCursor cur(range);
         for (int64_t i = 0; i < range.count; ++i, ++t, cur.next()) {
             const int sel = cur.sel, q = cur.qb * kTileQ + quarter * 32 + lane;
@@ -211,43 +162,18 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             const int va = rem >= 32 ? 32 : (rem > 0 ? static_cast<int>(rem) : 0);
             const int vb = rem >= 64 ? 32 : (rem > 32 ? static_cast<int>(rem) - 32 : 0);
             uint32_t ra[32], rb[32];
-            if (MODE != kModeDense) epi.begin_tile(q, q < a.nq);
-            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
-            if (ok) {
-                ptx::tc_fence_after();
-                const uint32_t tacc = tmem_base + (ab ? kAcc1 : 0u) + part * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
-                ptx::tmem_ld_32x32(tacc, ra);
-                ptx::tmem_ld_32x32(tacc + 32, rb);
-                ptx::tmem_ld_wait(ra);
-                ptx::tmem_ld_wait(rb);
-                ptx::tc_fence_before();
-                __syncwarp();
-                // shared columns: 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
-                if (lane == 0 && (ab ? part < 2 : part >= 2)) ptx::mbar_arrive(&bar_shared_free);
-            } else if (MODE != kModeDense) {
-                break;   // the host sees the error word
-            } else {
-                // nobody reads an error word behind a product: results that could not be computed are no numbers
-#pragma unroll
-                for (int c = 0; c < 32; ++c) ra[c] = rb[c] = 0x7fffffffu;
-            }
-            if (MODE == kModeDense) {
-                if (q < a.nq && va > 0) {
-                    const int64_t at = static_cast<int64_t>(q) * m.ldo + col0;
-                    const bool vec = m.vec != 0;
-                    if (m.dtype == kF32) {
-                        store_chunk(ra, static_cast<float*>(m.out) + at, va, vec);
-                        store_chunk(rb, static_cast<float*>(m.out) + at + 32, vb, vec);
-                    } else if (m.dtype == kF16) {
-                        store_chunk(ra, static_cast<__half*>(m.out) + at, va, vec);
-                        store_chunk(rb, static_cast<__half*>(m.out) + at + 32, vb, vec);
-                    } else {
-                        store_chunk(ra, static_cast<__nv_bfloat16*>(m.out) + at, va, vec);
-                        store_chunk(rb, static_cast<__nv_bfloat16*>(m.out) + at + 32, vb, vec);
-                    }
-                }
-                continue;
-            }
+            epi.begin_tile(q, q < a.nq);
+            if (!ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag)) break;
+            ptx::tc_fence_after();
+            const uint32_t tacc = tmem_base + (ab ? kAcc1 : 0u) + part * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
+            ptx::tmem_ld_32x32(tacc, ra);
+            ptx::tmem_ld_32x32(tacc + 32, rb);
+            ptx::tmem_ld_wait(ra);
+            ptx::tmem_ld_wait(rb);
+            ptx::tc_fence_before();
+            __syncwarp();
+            // shared columns: 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
+            if (lane == 0 && (ab ? part < 2 : part >= 2)) ptx::mbar_arrive(&bar_shared_free);
             if (MODE == kModeAppend && !a.direct) {
                 const uint32_t* gn = gnorm + col0;
                 if (L2) {
@@ -265,7 +191,7 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
                 epi.end_tile(slot);
             }
         }
-        if (MODE != kModeDense) epi.finish();
+        epi.finish();
     }
 
     // After an abort, copies in flight get time to land before the CTA's shared memory is released.
@@ -280,7 +206,7 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, 512);
     }
-    if (MODE != kModeDense && threadIdx.x == 0 && abort_flag) atomicOr(a.err, kDevErrPipelineTimeout);
+    if (threadIdx.x == 0 && abort_flag) atomicOr(a.err, kDevErrPipelineTimeout);
 }
 
 template <int MODE, int BURST, bool L2>
@@ -309,27 +235,6 @@ cudaError_t launch_one(Mx4Args m, const CUtensorMap* mapA, const CUtensorMap* ma
 
 }  // namespace
 
-void launch_mx4_product(int dtype, const Mx4ProductArgs& p, int num_sms, cudaStream_t st) {
-    CUtensorMap map_a, map_b;
-    if (encode_mx4_map(&map_a, p.a_codes, p.m, p.d, kTileQ) != 0 || encode_mx4_map(&map_b, p.b_codes, p.n, p.d, kTileB) != 0)
-        throw std::runtime_error("cuTensorMapEncodeTiled failed for the rows of a product");
-    Mx4Args m{};
-    m.g.nq = static_cast<int>(p.m);
-    m.g.N = p.n;
-    m.g.d = p.d;
-    m.g.n_tiles_total = m.g.n_tiles_sel = div_up(p.n, kTileB);
-    m.a_scales = p.a_scales;
-    m.b_scales = p.b_scales;
-    m.nb = mx4_blocks(p.d);
-    m.ng = mx4_groups(p.d);
-    m.out = p.out;
-    m.ldo = p.ldo;
-    m.dtype = dtype;
-    const int size = dtype == kF32 ? 4 : 2;
-    m.vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * size % 16 == 0;
-    B200_CUDA_CHECK((launch_one<kModeDense, 32, false>(m, &map_a, &map_b, num_sms, st)));
-}
-
 cudaError_t launch_mx4_dist(const GemmLaunch& L, const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales,
                             const CUtensorMap* mapA, const CUtensorMap* mapB, cudaStream_t stream) {
     Mx4Args m{};
@@ -347,10 +252,6 @@ cudaError_t launch_mx4_dist(const GemmLaunch& L, const GemmArgs& a, const uint8_
                   : launch_one<kModeBurstMin, 8, false>(m, mapA, mapB, L.num_sms, stream);
     return l2 ? launch_one<kModeBurstMin, 32, true>(m, mapA, mapB, L.num_sms, stream)
               : launch_one<kModeBurstMin, 32, false>(m, mapA, mapB, L.num_sms, stream);
-}
-
-int encode_mx4_map(CUtensorMap* out, const uint8_t* codes, int64_t rows, int d, int box_rows) {
-    return encode_rows_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, static_cast<int>(mx4_pitch(d)), box_rows);
 }
 
 }  // namespace b200

@@ -1,0 +1,526 @@
+// All scores of two sets of microscaled 4-bit rows, with tcgen05.mma kind::mxf4.
+//
+// out[i][j] is stored with j along a row, so the rows of b are the M side of the product (the 128 lanes of an
+// accumulator) and the rows of a its N side (TN columns): a store instruction of a warp then covers 32 neighbouring
+// outputs, whatever the output's stride is, and nothing passes through shared memory.  TN follows from m, so that few
+// rows of a cost little shared memory and leave the stage ring to the rows of b, which is what is read most.
+//   warp 0            : producer.  Per K chunk of 128 bytes (256 elements) 128 rows of b, TN rows of a and their
+//                       scales, which lie in memory in the order the tensor core wants.
+//   warp 1            : scales to TMEM (tcgen05.cp, a slot of columns per stage), up to four products of K = 64.
+//   other warps       : epilogue.  Thread = (row of b, up to 64 rows of a).
+// Two accumulators in turn.  Of 512 TMEM columns two of 256 would leave none for the scales: at TN = 256 they share
+// 96 columns (0-255 and 160-415), and tile t + 1 starts once tile t's shared columns are in registers.
+// Few tiles with a long K are split along K over a cluster, whose CTAs add their parts through shared memory in a
+// fixed order.
+#include "mx4_gemm.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <type_traits>
+
+#include "ptx_sm100.cuh"
+#include "row_ops.cuh"
+#include "smem_limit.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kLanes = 128;                     // rows of b in a tile
+constexpr int kChunk = 128;                     // bytes of codes of a row in a stage
+constexpr int kMaxStages = 10;
+constexpr int kSmemMost = 224 * 1024;
+constexpr int kMaxSplit = 8;
+
+template <int TN>
+struct Tile {
+    static constexpr int kBBytes = kLanes * kChunk, kABytes = TN * kChunk;
+    static constexpr int kGranulesA = TN > 128 ? 2 : 1;         // 128 rows of scales each
+    static constexpr int kScaleBytes = 1024 * (1 + kGranulesA); // two groups of 128 elements
+    static constexpr int kStage = kBBytes + kABytes + kScaleBytes;
+    static constexpr int kFit = (kSmemMost - 1024) / kStage;
+    static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kEpiWarps = TN > 64 ? TN / 16 : 4;
+    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    static constexpr int kCols = TN > 64 ? 64 : TN;              // columns of an epilogue thread
+    static constexpr uint32_t kAcc1 = TN == 256 ? 160 : TN;      // second accumulator
+    static constexpr uint32_t kSlotGroup = 4 + 4 * kGranulesA;   // TMEM columns of a group's scales
+    static constexpr uint32_t kSlot = 2 * kSlotGroup;
+    static constexpr uint32_t kScaleCol = TN == 256 ? 416 : 2 * TN;
+    static_assert(kScaleCol + kStages * kSlot <= 512, "TMEM columns");
+};
+
+struct ProductArgs {
+    const uint8_t* a_scales;
+    const uint8_t* b_scales;
+    int nb, ng;              // blocks of a row, groups of four
+    int64_t m, n;
+    void* out;
+    int64_t ldo;
+    int a_tiles, b_tiles;    // tiles of TN rows of a, of 128 rows of b
+    int split;               // CTAs of a cluster that share a tile's K (1: none)
+};
+
+__device__ __forceinline__ void next_tile(const ProductArgs& p, int& bt, int& at) {
+    if (++at == p.a_tiles) {
+        at = 0;
+        ++bt;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_one(T* o, float v) {
+    if constexpr (std::is_same<T, float>::value) *o = v;
+    else if constexpr (std::is_same<T, __half>::value) *o = __float2half_rn(v);
+    else *o = __float2bfloat16_rn(v);
+}
+
+// The end of a CTA: TMEM goes back; a split tile (bt, at), whose parts lie in shared memory as [TN][128], is added up.
+template <int THREADS, int TN, typename T>
+__device__ __forceinline__ void finish(const ProductArgs& p, int warp, uint32_t tmem_base, volatile int& abort_flag, uint8_t* smem,
+                                       int bt, int at, int part) {
+    // After an abort, copies in flight get time to land before the shared memory is used again or released.
+    __syncwarp();
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) { }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, 512);
+    }
+    if (p.split > 1) {
+        ptx::cluster_sync();
+        // this CTA's share of the tile's columns: the parts in order of K
+        const int c0 = TN * part / p.split, c1 = TN * (part + 1) / p.split;
+        uint32_t peer[kMaxSplit];
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r) peer[r] = r < p.split ? ptx::cluster_addr(ptx::smem_u32(smem), r) : 0u;
+        for (int e = c0 * kLanes + threadIdx.x; e < c1 * kLanes; e += THREADS) {
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < kMaxSplit; ++r)
+                if (r < p.split) v += ptx::cluster_load(peer[r] + e * 4);
+            const int64_t i = static_cast<int64_t>(at) * TN + e / kLanes, j = static_cast<int64_t>(bt) * kLanes + e % kLanes;
+            if (i < p.m && j < p.n) store_one(static_cast<T*>(p.out) + i * p.ldo + j, v);
+        }
+        ptx::cluster_sync();   // (the parts stay until everybody has read them)
+    }
+}
+
+template <int TN, typename T>
+__global__ void __launch_bounds__(Tile<TN>::kThreads, 1)
+mx4_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+                   const __grid_constant__ ProductArgs p) {
+    using K = Tile<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[K::kStages], bar_empty[K::kStages], bar_acc_full[2], bar_acc_free[2];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int chunks = (p.ng + 1) / 2;
+    // this CTA's tiles (in order of b, so that a tile's rows of b are read again from close by) and chunks of K
+    const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;
+    const int workers = gridDim.x / p.split, worker = blockIdx.x / p.split;
+    const int64_t lo = total * worker / workers, hi = total * (worker + 1) / workers;
+    const int part = p.split > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
+    const int kc0 = chunks * part / p.split, kc1 = chunks * (part + 1) / p.split;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < K::kStages; ++s) {
+            ptx::mbar_init(&bar_full[s], 1);
+            ptx::mbar_init(&bar_empty[s], 1);
+        }
+        ptx::mbar_init(&bar_acc_full[0], 1);
+        ptx::mbar_init(&bar_acc_full[1], 1);
+        // TN = 256: one for both accumulators, told by the warps that hold columns which both have
+        ptx::mbar_init(&bar_acc_free[0], TN == 256 ? K::kEpiWarps / 2 : K::kEpiWarps);
+        ptx::mbar_init(&bar_acc_free[1], K::kEpiWarps);
+        abort_flag = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&map_a);
+        ptx::prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&tmem_base_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+
+    if (warp == 0) {
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        const int64_t a_granules = (p.m + 127) / 128;
+        int bt = static_cast<int>(lo / p.a_tiles), at = static_cast<int>(lo % p.a_tiles);
+        for (int64_t i = lo; i < hi && ok; ++i, next_tile(p, bt, at)) {
+            const bool second = K::kGranulesA > 1 && 2 * at + 1 < a_granules;   // the upper 128 rows of a exist
+            const uint8_t* sb = p.b_scales + static_cast<int64_t>(bt) * p.ng * 512;
+            const uint8_t* sa = p.a_scales + static_cast<int64_t>(K::kGranulesA * at) * p.ng * 512;
+            for (int kc = kc0; kc < kc1; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (leader) {
+                    uint8_t* st = smem + s * K::kStage;
+                    uint8_t* sf = st + K::kBBytes + K::kABytes;
+                    const uint32_t bytes = min(2, p.ng - 2 * kc) * 512u;
+                    ptx::mbar_expect_tx(&bar_full[s], K::kBBytes + K::kABytes + bytes * (second ? 3u : 2u));
+                    ptx::tma_load_2d(st, &map_b, &bar_full[s], kc * kChunk, bt * kLanes);
+                    ptx::tma_load_2d(st + K::kBBytes, &map_a, &bar_full[s], kc * kChunk, at * TN);
+                    ptx::bulk_load_1d(sf, sb + kc * 1024, bytes, &bar_full[s]);
+                    ptx::bulk_load_1d(sf + 1024, sa + kc * 1024, bytes, &bar_full[s]);
+                    if (second) ptx::bulk_load_1d(sf + 2048, sa + p.ng * 512 + kc * 1024, bytes, &bar_full[s]);
+                }
+                __syncwarp();
+                if (++s == K::kStages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kLanes, TN, 0), kIdesc2 = ptx::umma_idesc_mxf4(kLanes, TN, 2);
+        const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
+        const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
+        const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0, t = 0;
+        bool ok = true;
+        for (int64_t i = lo; i < hi && ok; ++i, ++t) {
+            // TN = 256: tile t - 1's shared columns (and with them all of tile t - 2); else tile t - 2
+            if (TN == 256 ? t >= 1 && !ptx::mbar_wait_warp(&bar_acc_free[0], (t - 1) & 1u, &abort_flag)
+                          : t >= 2 && !ptx::mbar_wait_warp(&bar_acc_free[t & 1u], ((t >> 1) - 1) & 1u, &abort_flag)) { ok = false; break; }
+            const uint32_t tacc = tmem_base + (t & 1u ? K::kAcc1 : 0u);
+            for (int kc = kc0; kc < kc1; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+                ptx::tc_fence_after();
+                const uint32_t st = ring_lo + s * (K::kStage >> 4);
+                const uint32_t sf_lo = st + ((K::kBBytes + K::kABytes) >> 4);
+                const uint32_t slot = tmem_base + K::kScaleCol + s * K::kSlot;
+                const int steps = min(4, (p.nb - 8 * kc + 1) / 2);   // 64 elements each
+                if (leader) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        if (2 * g < steps)
+#pragma unroll
+                            for (int h = 0; h < 1 + K::kGranulesA; ++h)
+                                ptx::tmem_cp_scales(slot + g * K::kSlotGroup + 4 * h, sf_hi | static_cast<uint64_t>(sf_lo + 64 * h + 32 * g));
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t col = slot + (ks >> 1) * K::kSlotGroup;
+                        if (ks < steps)
+                            ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                           desc_hi | static_cast<uint64_t>(st + (K::kBBytes >> 4) + ks * 2),
+                                           (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc > kc0 || ks) ? 1u : 0u);
+                    }
+                    ptx::umma_commit(&bar_empty[s]);
+                    if (kc + 1 == kc1) ptx::umma_commit(&bar_acc_full[t & 1u]);
+                }
+                __syncwarp();
+                if (++s == K::kStages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, group = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
+        uint32_t t = 0;
+        bool ok = true;
+        float* parts = reinterpret_cast<float*>(smem);           // split: [TN][128]
+        int bt = static_cast<int>(lo / p.a_tiles), at = static_cast<int>(lo % p.a_tiles);
+        for (int64_t i = lo; i < hi; ++i, ++t, next_tile(p, bt, at)) {
+            const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
+            const int64_t i0 = static_cast<int64_t>(at) * TN + group * K::kCols;
+            const uint32_t ab = t & 1u;
+            uint32_t r[K::kCols];
+            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
+            if (ok) {
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + (ab ? K::kAcc1 : 0u) + group * K::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+                if constexpr (K::kCols >= 32) {
+#pragma unroll
+                    for (int c = 0; c < K::kCols; c += 32) ptx::tmem_ld_32x32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+#pragma unroll
+                    for (int c = 0; c < K::kCols; c += 32) ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+                } else {
+                    ptx::tmem_ld_32x16(tacc, r);
+                    ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[16]>(r));
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                // TN = 256: shared are 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
+                if (lane == 0 && (TN != 256 || (ab ? group < 2 : group >= 2))) ptx::mbar_arrive(&bar_acc_free[TN == 256 ? 0 : ab]);
+            } else {
+                // nobody reads an error word behind a product: results that could not be computed are no numbers
+#pragma unroll
+                for (int c = 0; c < K::kCols; ++c) r[c] = 0x7fffffffu;
+            }
+            if (p.split > 1) {   // (one tile)  every load of the ring has been consumed: it holds the part now
+#pragma unroll
+                for (int c = 0; c < K::kCols; ++c) parts[(group * K::kCols + c) * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
+                continue;
+            }
+            const int cols = static_cast<int>(min(p.m - i0, static_cast<int64_t>(K::kCols)));
+            if (j < p.n) {
+                T* o = static_cast<T*>(p.out) + i0 * p.ldo + j;
+                if (cols >= K::kCols) {
+#pragma unroll
+                    for (int c = 0; c < K::kCols; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < K::kCols; ++c, o += p.ldo)
+                        if (c < cols) store_one(o, __uint_as_float(r[c]));
+                }
+            }
+        }
+    }
+
+    finish<K::kThreads, TN, T>(p, warp, tmem_base, abort_flag, smem, static_cast<int>(lo / p.a_tiles), static_cast<int>(lo % p.a_tiles), part);
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows of a (up to 64): they and their scales stay in shared memory and in TMEM, only rows of b travel through
+// the ring, and four accumulators with an epilogue of four warps each keep four tiles on the way -- with one row of a
+// a tile is little work for anybody, and what counts is how many of the hand-offs between the roles overlap.
+// ---------------------------------------------------------------------------------------
+constexpr int kFewStage = kLanes * kChunk + 1024;
+constexpr int kFewMaxStages = 12;
+constexpr int kFewAcc = 4;
+constexpr int kFewThreads = 64 + 128 * kFewAcc;
+template <int TN>
+constexpr int kFewMaxChunks = TN == 64 ? 16 : 32;   // TMEM columns: accumulators, 8 a chunk of a's scales, 8 a stage
+static_assert(kFewAcc * 64 + 8 * kFewMaxChunks<64> + 8 * kFewMaxStages <= 512 && kFewAcc * 32 + 8 * kFewMaxChunks<32> + 8 * kFewMaxStages <= 512,
+              "TMEM columns");
+template <int TN>
+constexpr int few_resident_bytes(int chunks) { return chunks * (TN * kChunk + 1024); }
+
+template <int TN, typename T>
+__global__ void __launch_bounds__(kFewThreads, 1)
+mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+               const __grid_constant__ ProductArgs p, const int stages) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[kFewMaxStages], bar_empty[kFewMaxStages], bar_acc_full[kFewAcc], bar_acc_free[kFewAcc], bar_a;
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int chunks = (p.ng + 1) / 2;
+    const int workers = gridDim.x / p.split, worker = blockIdx.x / p.split;
+    const int lo = static_cast<int>(static_cast<int64_t>(p.b_tiles) * worker / workers);
+    const int hi = static_cast<int>(static_cast<int64_t>(p.b_tiles) * (worker + 1) / workers);
+    const int part = p.split > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
+    const int kc0 = chunks * part / p.split, kc1 = chunks * (part + 1) / p.split, nkc = kc1 - kc0;
+    uint8_t* a_codes = smem;                              // [nkc][TN][128 B]
+    uint8_t* a_scales = smem + nkc * TN * kChunk;         // [nkc][1 KB]
+    uint8_t* ring = a_scales + nkc * 1024;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            ptx::mbar_init(&bar_full[s], 1);
+            ptx::mbar_init(&bar_empty[s], 1);
+        }
+        for (int b = 0; b < kFewAcc; ++b) {
+            ptx::mbar_init(&bar_acc_full[b], 1);
+            ptx::mbar_init(&bar_acc_free[b], 4);
+        }
+        ptx::mbar_init(&bar_a, 1);
+        abort_flag = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&map_a);
+        ptx::prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&tmem_base_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+    const uint32_t col_a = tmem_base + kFewAcc * TN, col_b = col_a + 8 * nkc;
+
+    if (warp == 0) {
+        const bool leader = ptx::elect_one();
+        const uint32_t a_sf = static_cast<uint32_t>(min(p.ng, 2 * kc1) - 2 * kc0) * 512u;
+        if (leader) {
+            ptx::mbar_expect_tx(&bar_a, static_cast<uint32_t>(nkc) * TN * kChunk + a_sf);
+            for (int kc = kc0; kc < kc1; ++kc) ptx::tma_load_2d(a_codes + (kc - kc0) * TN * kChunk, &map_a, &bar_a, kc * kChunk, 0);
+            ptx::bulk_load_1d(a_scales, p.a_scales + kc0 * 1024, a_sf, &bar_a);
+        }
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (int bt = lo; bt < hi && ok; ++bt) {
+            const uint8_t* sb = p.b_scales + static_cast<int64_t>(bt) * p.ng * 512;
+            for (int kc = kc0; kc < kc1; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (leader) {
+                    uint8_t* st = ring + s * kFewStage;
+                    const uint32_t bytes = min(2, p.ng - 2 * kc) * 512u;
+                    ptx::mbar_expect_tx(&bar_full[s], kLanes * kChunk + bytes);
+                    ptx::tma_load_2d(st, &map_b, &bar_full[s], kc * kChunk, bt * kLanes);
+                    ptx::bulk_load_1d(st + kLanes * kChunk, sb + kc * 1024, bytes, &bar_full[s]);
+                }
+                __syncwarp();
+                if (++s == static_cast<uint32_t>(stages)) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kLanes, TN, 0), kIdesc2 = ptx::umma_idesc_mxf4(kLanes, TN, 2);
+        const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
+        const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
+        const uint32_t a_lo = (ptx::smem_u32(a_codes) & 0x3FFFFu) >> 4, ring_lo = (ptx::smem_u32(ring) & 0x3FFFFu) >> 4;
+        const uint32_t a_sf_lo = (ptx::smem_u32(a_scales) & 0x3FFFFu) >> 4;
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0, t = 0;
+        bool ok = ptx::mbar_wait_warp(&bar_a, 0u, &abort_flag);
+        ptx::tc_fence_after();
+        if (ok && leader)
+            for (int g = 0; g < min(p.ng, 2 * kc1) - 2 * kc0; ++g) ptx::tmem_cp_scales(col_a + 4 * g, sf_hi | static_cast<uint64_t>(a_sf_lo + 32 * g));
+        __syncwarp();
+        for (int bt = lo; bt < hi && ok; ++bt, ++t) {
+            const uint32_t ab = t % kFewAcc;
+            if (t >= kFewAcc && !ptx::mbar_wait_warp(&bar_acc_free[ab], (t / kFewAcc - 1) & 1u, &abort_flag)) { ok = false; break; }
+            const uint32_t tacc = tmem_base + ab * TN;
+            for (int kc = kc0; kc < kc1; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+                ptx::tc_fence_after();
+                const uint32_t st = ring_lo + s * (kFewStage >> 4), slot = col_b + s * 8;
+                const uint32_t at = a_lo + (kc - kc0) * (TN * kChunk >> 4), sa = col_a + (kc - kc0) * 8;
+                const int steps = min(4, (p.nb - 8 * kc + 1) / 2);   // 64 elements each
+                if (leader) {
+                    ptx::tmem_cp_scales(slot, sf_hi | static_cast<uint64_t>(st + (kLanes * kChunk >> 4)));
+                    if (steps > 2) ptx::tmem_cp_scales(slot + 4, sf_hi | static_cast<uint64_t>(st + (kLanes * kChunk >> 4) + 32));
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        if (ks < steps)
+                            ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2), desc_hi | static_cast<uint64_t>(at + ks * 2),
+                                           (ks & 1) ? kIdesc2 : kIdesc0, slot + (ks >> 1) * 4, sa + (ks >> 1) * 4, (kc > kc0 || ks) ? 1u : 0u);
+                    ptx::umma_commit(&bar_empty[s]);
+                    if (kc + 1 == kc1) ptx::umma_commit(&bar_acc_full[ab]);
+                }
+                __syncwarp();
+                if (++s == static_cast<uint32_t>(stages)) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, group = (warp - 2) >> 2;   // TMEM lanes; every fourth tile
+        bool ok = true;
+        float* parts = reinterpret_cast<float*>(smem);           // split: [TN][128]
+        uint32_t turn = 0;
+        for (int bt = lo + group; bt < hi; bt += kFewAcc, ++turn) {
+            const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
+            uint32_t r[TN];
+            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[group], turn & 1u, &abort_flag);
+            if (ok) {
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + group * TN + (static_cast<uint32_t>(quarter * 32) << 16);
+                if constexpr (TN >= 32) {
+#pragma unroll
+                    for (int c = 0; c < TN; c += 32) ptx::tmem_ld_32x32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+#pragma unroll
+                    for (int c = 0; c < TN; c += 32) ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+                } else {
+                    ptx::tmem_ld_32x16(tacc, r);
+                    ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[16]>(r));
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bar_acc_free[group]);
+            } else {
+                // (as above: no numbers)
+#pragma unroll
+                for (int c = 0; c < TN; ++c) r[c] = 0x7fffffffu;
+            }
+            if (p.split > 1) {
+                // (one tile: its commit says that every copy and product has read what lies there)
+#pragma unroll
+                for (int c = 0; c < TN; ++c) parts[c * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
+                continue;
+            }
+            const int cols = static_cast<int>(p.m);
+            if (j < p.n) {
+                T* o = static_cast<T*>(p.out) + j;
+#pragma unroll
+                for (int c = 0; c < TN; ++c, o += p.ldo)
+                    if (c < cols) store_one(o, __uint_as_float(r[c]));
+            }
+        }
+    }
+
+    finish<kFewThreads, TN, T>(p, warp, tmem_base, abort_flag, smem, lo, 0, part);
+}
+
+template <int TN, typename T>
+void launch(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
+    using K = Tile<TN>;
+    CUtensorMap map_a, map_b;
+    if (encode_mx4_map(&map_a, q.a_codes, q.m, q.d, TN) != 0 || encode_mx4_map(&map_b, q.b_codes, q.n, q.d, kLanes) != 0)
+        throw std::runtime_error("cuTensorMapEncodeTiled failed for the rows of a product");
+    ProductArgs p{};
+    p.a_scales = q.a_scales;
+    p.b_scales = q.b_scales;
+    p.nb = mx4_blocks(q.d);
+    p.ng = mx4_groups(q.d);
+    p.m = q.m;
+    p.n = q.n;
+    p.out = q.out;
+    p.ldo = q.ldo;
+    p.a_tiles = div_up(q.m, TN);
+    p.b_tiles = div_up(q.n, kLanes);
+    const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;
+    p.split = 1;
+    const int chunks = (p.ng + 1) / 2;
+    while (p.split < kMaxSplit && total * p.split * 2 <= num_sms && p.split * 2 <= chunks) p.split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.split > 1 ? total * p.split : std::min<int64_t>(total, num_sms)));
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(p.split);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.split > 1 ? 1 : 0;
+    if constexpr (TN <= 64) {
+        const int mine = (chunks + p.split - 1) / p.split;   // chunks of K of a CTA
+        const int stages = std::min(kFewMaxStages, (kSmemMost - 1024 - few_resident_bytes<TN>(mine)) / kFewStage);
+        if (mine <= kFewMaxChunks<TN> && stages >= 4) {
+            auto kern = mx4_few_kernel<TN, T>;
+            B200_CUDA_CHECK(allow_max_smem(kern));
+            cfg.blockDim = dim3(kFewThreads);
+            cfg.dynamicSmemBytes = 1024 + few_resident_bytes<TN>(mine) + stages * kFewStage;
+            B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p, stages));
+            return;
+        }
+    }
+    auto kern = mx4_product_kernel<TN, T>;
+    B200_CUDA_CHECK(allow_max_smem(kern));
+    cfg.blockDim = dim3(K::kThreads);
+    cfg.dynamicSmemBytes = K::kSmem;
+    B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p));
+}
+
+template <typename T>
+void product(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
+    if (q.m <= 16) launch<16, T>(q, num_sms, st);
+    else if (q.m <= 32) launch<32, T>(q, num_sms, st);
+    else if (q.m <= 64) launch<64, T>(q, num_sms, st);
+    else if (q.m <= 128) launch<128, T>(q, num_sms, st);
+    else launch<256, T>(q, num_sms, st);
+}
+
+}  // namespace
+
+void launch_mx4_product(int dtype, const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
+    if (dtype == kF32) product<float>(q, num_sms, st);
+    else if (dtype == kF16) product<__half>(q, num_sms, st);
+    else product<__nv_bfloat16>(q, num_sms, st);
+}
+
+int encode_mx4_map(CUtensorMap* out, const uint8_t* codes, int64_t rows, int d, int box_rows) {
+    return encode_rows_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, static_cast<int>(mx4_pitch(d)), box_rows);
+}
+
+}  // namespace b200
