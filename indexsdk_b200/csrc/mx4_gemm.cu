@@ -2,11 +2,11 @@
 // selection in the epilogue.
 //
 // A CTA computes 128 x 256 tiles (queries x base rows) of fp32 accumulators in TMEM:
-//   warp 0 (one lane)  : producer.  Per K chunk of 128 bytes (256 elements) two tensor copies (128 and 256 rows,
+//   warp 0             : producer.  Per K chunk of 128 bytes (256 elements) two tensor copies (128 and 256 rows,
 //                        SWIZZLE_128B) and up to three copies of scales into a ring of four 51 KB stages.  The
 //                        scales lie in memory in the order the tensor core wants, 512 bytes for 128 rows x 4
 //                        blocks, so nothing is rearranged on the way.
-//   warp 1 (one lane)  : copies a stage's scales into TMEM (tcgen05.cp, a slot of 24 columns per stage) and issues
+//   warp 1             : copies a stage's scales into TMEM (tcgen05.cp, a slot of 24 columns per stage) and issues
 //                        up to four 128 x 256 x 64 products.
 //   warps 2-17         : epilogue.  Thread = (row, 64 of the tile's 256 columns), both 32-column chunks in
 //                        registers at once, so that the accumulator goes back before the slow part begins.
@@ -80,18 +80,19 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
     const ItemRange range(a, n_qb);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t s = 0, ph = 0;
-            bool ok = true;
-            ItemCursor cur(range);
-            const int64_t b_granules = (a.N + 127) / 128;
-            for (int64_t i = 0; i < range.count && ok; ++i, cur.next()) {
-                const int64_t tile = tile_of(a, cur.sel);
-                const bool second = 2 * tile + 1 < b_granules;   // the tile's upper 128 rows exist
-                const uint8_t* sa = m.a_scales + static_cast<int64_t>(cur.qb) * m.ng * 512;
-                const uint8_t* sb = m.b_scales + 2 * tile * m.ng * 512;
-                for (int kc = 0; kc < nkc; ++kc) {
-                    if (!ptx::mbar_wait_bounded(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        ItemCursor cur(range);
+        const int64_t b_granules = (a.N + 127) / 128;
+        for (int64_t i = 0; i < range.count && ok; ++i, cur.next()) {
+            const int64_t tile = tile_of(a, cur.sel);
+            const bool second = 2 * tile + 1 < b_granules;   // the tile's upper 128 rows exist
+            const uint8_t* sa = m.a_scales + static_cast<int64_t>(cur.qb) * m.ng * 512;
+            const uint8_t* sb = m.b_scales + 2 * tile * m.ng * 512;
+            for (int kc = 0; kc < nkc; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (leader) {
                     uint8_t* st = smem + s * kStageBytes;
                     const uint32_t sf = min(2, m.ng - 2 * kc) * 512u;
                     ptx::mbar_expect_tx(&bar_full[s], kABytes + kBBytes + sf * (second ? 3u : 2u));
@@ -101,50 +102,52 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
                     ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes, sb + kc * 1024, sf, &bar_full[s]);
                     if (second)
                         ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes + 1024, sb + m.ng * 512 + kc * 1024, sf, &bar_full[s]);
-                    if (++s == kStages) { s = 0; ph ^= 1u; }
                 }
+                __syncwarp();
+                if (++s == kStages) { s = 0; ph ^= 1u; }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 0), kIdesc2 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 2);
-            const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
-            const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
-            const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
-            uint32_t s = 0, ph = 0, t = 0;
-            bool ok = true;
-            for (int64_t i = 0; i < range.count && ok; ++i, ++t) {
-                // the columns this accumulator shares with tile t - 1's (and with them all of tile t - 2's)
-                if (t && !ptx::mbar_wait_bounded(&bar_shared_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
+        constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 0), kIdesc2 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 2);
+        const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
+        const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
+        const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0, t = 0;
+        bool ok = true;
+        for (int64_t i = 0; i < range.count && ok; ++i, ++t) {
+            // the columns this accumulator shares with tile t - 1's (and with them all of tile t - 2's)
+            if (t && !ptx::mbar_wait_warp(&bar_shared_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
+            const uint32_t tacc = tmem_base + (t & 1u ? kAcc1 : 0u);
+            for (int kc = 0; kc < nkc; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
                 ptx::tc_fence_after();
-                const uint32_t tacc = tmem_base + (t & 1u ? kAcc1 : 0u);
-                for (int kc = 0; kc < nkc; ++kc) {
-                    if (!ptx::mbar_wait_bounded(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
-                    ptx::tc_fence_after();
-                    const uint32_t st = ring_lo + s * (kStageBytes >> 4);
-                    const uint32_t sf_lo = st + ((kABytes + kBBytes) >> 4);
-                    const uint32_t slot = tmem_base + kScaleCols + s * kScaleSlot;
-                    const int groups = min(2, m.ng - 2 * kc);
-                    for (int g = 0; g < groups; ++g) {   // slot: 4 columns of a's scales, 8 of b's, per group
+                const uint32_t st = ring_lo + s * (kStageBytes >> 4);
+                const uint32_t sf_lo = st + ((kABytes + kBBytes) >> 4);
+                const uint32_t slot = tmem_base + kScaleCols + s * kScaleSlot;
+                const int steps = min(4, (m.nb - 8 * kc + 1) / 2);   // 64 elements each
+                if (leader) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {   // slot: 4 columns of a's scales, 8 of b's, per group
+                        if (2 * g >= steps) continue;
                         const uint32_t col = slot + g * 12;
                         ptx::tmem_cp_scales(col, sf_hi | static_cast<uint64_t>(sf_lo + g * 32));
                         ptx::tmem_cp_scales(col + 4, sf_hi | static_cast<uint64_t>(sf_lo + 64 + g * 32));
                         ptx::tmem_cp_scales(col + 8, sf_hi | static_cast<uint64_t>(sf_lo + 128 + g * 32));
                     }
-                    const int steps = min(4, (m.nb - 8 * kc + 1) / 2);   // 64 elements each
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
-                        if (ks >= steps) break;
                         const uint32_t col = slot + (ks >> 1) * 12;
-                        ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
-                                       desc_hi | static_cast<uint64_t>(st + (kABytes >> 4) + ks * 2),
-                                       (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
+                        if (ks < steps)
+                            ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                           desc_hi | static_cast<uint64_t>(st + (kABytes >> 4) + ks * 2),
+                                           (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
                     }
                     ptx::umma_commit(&bar_empty[s]);
-                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                    if (kc + 1 == nkc) ptx::umma_commit(&bar_acc_full[t & 1u]);
                 }
-                if (!ok) break;
-                ptx::umma_commit(&bar_acc_full[t & 1u]);
+                __syncwarp();
+                if (++s == kStages) { s = 0; ph ^= 1u; }
             }
         }
     } else {
