@@ -2,17 +2,20 @@
 // selection in the epilogue.
 //
 // A CTA computes 128 x 256 tiles (queries x base rows) of fp32 accumulators in TMEM:
-//   warp 0             : producer.  Per K chunk of 128 bytes (256 elements) two tensor copies (128 and 256 rows,
-//                        SWIZZLE_128B) and up to three copies of scales into a ring of four 51 KB stages.  The
-//                        scales lie in memory in the order the tensor core wants, 512 bytes for 128 rows x 4
-//                        blocks, so nothing is rearranged on the way.
-//   warp 1             : copies a stage's scales into TMEM (tcgen05.cp, a slot of 24 columns per stage) and issues
-//                        up to four 128 x 256 x 64 products.
-//   warps 2-17         : epilogue.  Thread = (row, 64 of the tile's 256 columns), both 32-column chunks in
-//                        registers at once, so that the accumulator goes back before the slow part begins.
-// TMEM has 512 columns: two accumulators of 256 and the 96 columns of scales do not fit side by side.  The two
-// accumulators therefore SHARE 96 columns (0-255 and 160-415; scales 416-511): tile t + 1 may start once tile t's
-// shared columns are in registers, which half of the epilogue warps report.
+//   warps 0, 1  : producers of the even and the odd tiles, each with half of the ring.  Per K chunk of 128 bytes (256
+//                 elements) a tensor copy of 256 base rows (SWIZZLE_128B) and their scales, which lie in memory in
+//                 the order the tensor core wants, 512 bytes for 128 rows x 4 blocks, so nothing is rearranged.
+//                 Up to d = 1024 the query tile stays in shared memory and its scales in TMEM for a whole query
+//                 block: all CTAs fetching the same few rows again for every tile wait at the few L2 lines that
+//                 hold them (1 M x 128, 64 queries: 3 000 cycles a tile).  Longer rows travel through the ring.
+//   warps 2, 3  : MMA of the even and the odd tiles: a stage's scales into TMEM (tcgen05.cp, a slot of columns per
+//                 stage), up to four 128 x 256 x 64 products.  Two, because waiting and issuing take one warp longer
+//                 than the tensor pipe takes for a short K.
+//   warps 4-19  : epilogue.  Thread = (row, 64 of the tile's 256 columns), both 32-column chunks in
+//                 registers at once, so that the accumulator goes back before the slow part begins.
+// TMEM has 512 columns: two accumulators of 256 and the scales do not fit side by side.  The two accumulators
+// therefore SHARE 104 columns (0-255 and 152-407; scales 408-511): tile t + 1 may start once tile t's shared columns
+// are in registers, which half of the epilogue warps report.
 #include "mx4_gemm.cuh"
 
 #include <algorithm>
@@ -27,48 +30,68 @@
 namespace b200 {
 namespace {
 
-constexpr int kStages = 4;
 constexpr int kABytes = kTileQ * kChunkBytes, kBBytes = kTileB * kChunkBytes;   // 16 KB, 32 KB
 constexpr int kSfaBytes = 1024, kSfbBytes = 2048;                               // two groups of 128 elements
-constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;          // 51 KB
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kResidentChunks = 4;   // of the query tile
+constexpr int kMaxStages = 6;
+constexpr int kSmemMost = 224 * 1024;
 constexpr int kEpiWarps = 16;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr uint32_t kAcc1 = 160, kScaleCols = 416, kScaleSlot = 24;   // TMEM columns
+constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr uint32_t kAcc1 = 152, kScaleCols = 408, kAllScaleCols = 104;   // TMEM columns
+// A stage: base rows and their scales, or with them the queries and theirs.
+constexpr int stage_bytes(bool resident) { return kBBytes + kSfbBytes + (resident ? 0 : kABytes + kSfaBytes); }
+constexpr uint32_t scale_slot(bool resident) { return resident ? 16 : 24; }
+constexpr int half_stages(bool resident, int chunks) {   // of each pipe
+    const int kept = resident ? chunks : 0;
+    const int by_smem = (kSmemMost - 1024 - kept * (kABytes + kSfaBytes)) / stage_bytes(resident);
+    const int by_tmem = (static_cast<int>(kAllScaleCols) - 8 * kept) / static_cast<int>(scale_slot(resident));
+    const int n = by_smem < by_tmem ? by_smem : by_tmem;
+    return (n < kMaxStages ? n : kMaxStages) / 2;
+}
+static_assert(half_stages(true, 1) == 3 && half_stages(true, kResidentChunks) == 2 && half_stages(false, 8) == 2, "ring");
 
 struct Mx4Args {
     GemmArgs g;
     const uint8_t* a_scales;
     const uint8_t* b_scales;
     int nb, ng;      // blocks of a row, groups of four
+    int half;        // stages of a pipe
 };
 
-template <int MODE, int BURST, bool L2>
+template <int MODE, int BURST, bool L2, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, 1)
-mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Mx4Args m) {
+mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ Mx4Args m) {
     const GemmArgs& a = m.g;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bar_full[kStages], bar_empty[kStages], bar_acc_full[2], bar_shared_free;
+    __shared__ uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_acc_full[2], bar_shared_free[2];
+    __shared__ uint64_t bar_a_full, bar_a_scales, bar_a_free;   // RESIDENT: queries landed, their scales in TMEM, both read for the last time
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int nkc = (m.ng + 1) / 2;   // chunks of 256 elements
+    constexpr int kStage = stage_bytes(RESIDENT);
+    uint8_t* a_scales = smem + nkc * kABytes;                                   // RESIDENT: [nkc] codes, [nkc] scales, ring
+    uint8_t* ring = RESIDENT ? a_scales + nkc * kSfaBytes : smem;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < 2 * m.half; ++s) {
             ptx::mbar_init(&bar_full[s], 1);
             ptx::mbar_init(&bar_empty[s], 1);
         }
         ptx::mbar_init(&bar_acc_full[0], 1);
         ptx::mbar_init(&bar_acc_full[1], 1);
-        ptx::mbar_init(&bar_shared_free, kEpiWarps / 2);
+        ptx::mbar_init(&bar_shared_free[0], kEpiWarps / 2);
+        ptx::mbar_init(&bar_shared_free[1], kEpiWarps / 2);
+        ptx::mbar_init(&bar_a_full, 1);
+        ptx::mbar_init(&bar_a_scales, 1);
+        ptx::mbar_init(&bar_a_free, 2);
         abort_flag = 0;
         ptx::mbar_fence_init();
         ptx::prefetch_tensormap(&mapA);
         ptx::prefetch_tensormap(&mapB);
     }
-    if (warp == 1) {
+    if (warp == 2) {
         ptx::tmem_alloc(&tmem_base_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -78,80 +101,123 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
     const uint32_t tmem_base = tmem_base_slot;
     const int n_qb = (a.nq + kTileQ - 1) / kTileQ;
     const ItemRange range(a, n_qb);
+    const uint32_t pipe = warp & 1u, s0 = pipe * m.half;   // of producers and MMA warps
+    const uint32_t col_a = tmem_base + kScaleCols, col_b = col_a + (RESIDENT ? 8 * nkc : 0);
 
-    if (warp == 0) {
+    if (warp < 2) {
         const bool leader = ptx::elect_one();
-        uint32_t s = 0, ph = 0;
+        uint32_t s = 0, ph = 0, t = 0, loads = 0;
+        int cur_qb = -1;
         bool ok = true;
         ItemCursor cur(range);
         const int64_t b_granules = (a.N + 127) / 128;
-        for (int64_t i = 0; i < range.count && ok; ++i, cur.next()) {
-            const int64_t tile = tile_of(a, cur.sel);
-            const bool second = 2 * tile + 1 < b_granules;   // the tile's upper 128 rows exist
+        for (int64_t i = 0; i < range.count && ok; ++i, ++t, cur.next()) {
             const uint8_t* sa = m.a_scales + static_cast<int64_t>(cur.qb) * m.ng * 512;
-            const uint8_t* sb = m.b_scales + 2 * tile * m.ng * 512;
-            for (int kc = 0; kc < nkc; ++kc) {
-                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+            if (RESIDENT && pipe == 0 && cur.qb != cur_qb) {
+                if (loads && !ptx::mbar_wait_warp(&bar_a_free, (loads - 1u) & 1u, &abort_flag)) { ok = false; break; }
                 if (leader) {
-                    uint8_t* st = smem + s * kStageBytes;
-                    const uint32_t sf = min(2, m.ng - 2 * kc) * 512u;
-                    ptx::mbar_expect_tx(&bar_full[s], kABytes + kBBytes + sf * (second ? 3u : 2u));
-                    ptx::tma_load_2d(st, &mapA, &bar_full[s], kc * kChunkBytes, cur.qb * kTileQ);
-                    ptx::tma_load_2d(st + kABytes, &mapB, &bar_full[s], kc * kChunkBytes, static_cast<int>(tile * kTileB));
-                    ptx::bulk_load_1d(st + kABytes + kBBytes, sa + kc * 1024, sf, &bar_full[s]);
-                    ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes, sb + kc * 1024, sf, &bar_full[s]);
-                    if (second)
-                        ptx::bulk_load_1d(st + kABytes + kBBytes + kSfaBytes + 1024, sb + m.ng * 512 + kc * 1024, sf, &bar_full[s]);
+                    ptx::mbar_expect_tx(&bar_a_full, nkc * kABytes + m.ng * 512u);
+                    for (int kc = 0; kc < nkc; ++kc) ptx::tma_load_2d(smem + kc * kABytes, &mapA, &bar_a_full, kc * kChunkBytes, cur.qb * kTileQ);
+                    ptx::bulk_load_1d(a_scales, sa, m.ng * 512u, &bar_a_full);
                 }
                 __syncwarp();
-                if (++s == kStages) { s = 0; ph ^= 1u; }
+                ++loads;
+                cur_qb = cur.qb;
+            }
+            if ((t & 1u) != pipe) continue;
+            const int64_t tile = tile_of(a, cur.sel);
+            const bool second = 2 * tile + 1 < b_granules;   // the tile's upper 128 rows exist
+            const uint8_t* sb = m.b_scales + 2 * tile * m.ng * 512;
+            for (int kc = 0; kc < nkc; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_empty[s0 + s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (leader) {
+                    uint8_t* st = ring + (s0 + s) * kStage;
+                    uint8_t* sf = st + kBBytes;
+                    uint64_t* full = &bar_full[s0 + s];
+                    const uint32_t bytes = min(2, m.ng - 2 * kc) * 512u;
+                    ptx::mbar_expect_tx(full, kBBytes + bytes * (second ? 2u : 1u) + (RESIDENT ? 0u : kABytes + bytes));
+                    ptx::tma_load_2d(st, &mapB, full, kc * kChunkBytes, static_cast<int>(tile * kTileB));
+                    ptx::bulk_load_1d(sf, sb + kc * 1024, bytes, full);
+                    if (second) ptx::bulk_load_1d(sf + 1024, sb + m.ng * 512 + kc * 1024, bytes, full);
+                    if (!RESIDENT) {
+                        ptx::tma_load_2d(st + kBBytes + kSfbBytes, &mapA, full, kc * kChunkBytes, cur.qb * kTileQ);
+                        ptx::bulk_load_1d(st + kBBytes + kSfbBytes + kABytes, sa + kc * 1024, bytes, full);
+                    }
+                }
+                __syncwarp();
+                if (++s == static_cast<uint32_t>(m.half)) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 1) {
+    } else if (warp < 4) {
         constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 0), kIdesc2 = ptx::umma_idesc_mxf4(kTileQ, kTileB, 2);
         const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
         const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
-        const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
+        const uint32_t a_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4, ring_lo = (ptx::smem_u32(ring) & 0x3FFFFu) >> 4;
+        const uint32_t a_sf_lo = (ptx::smem_u32(a_scales) & 0x3FFFFu) >> 4;
         const bool leader = ptx::elect_one();
-        uint32_t s = 0, ph = 0, t = 0;
+        uint32_t s = 0, ph = 0, t = 0, seen = 0;
+        int cur_qb = -1;
         bool ok = true;
-        for (int64_t i = 0; i < range.count && ok; ++i, ++t) {
-            // the columns this accumulator shares with tile t - 1's (and with them all of tile t - 2's)
-            if (t && !ptx::mbar_wait_warp(&bar_shared_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
-            const uint32_t tacc = tmem_base + (t & 1u ? kAcc1 : 0u);
-            for (int kc = 0; kc < nkc; ++kc) {
-                if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+        ItemCursor cur(range);
+        for (int64_t i = 0; i < range.count && ok; ++i, ++t, cur.next()) {
+            if (RESIDENT && cur.qb != cur_qb) {
+                if (!ptx::mbar_wait_warp(&bar_a_full, seen & 1u, &abort_flag)) { ok = false; break; }
                 ptx::tc_fence_after();
-                const uint32_t st = ring_lo + s * (kStageBytes >> 4);
-                const uint32_t sf_lo = st + ((kABytes + kBBytes) >> 4);
-                const uint32_t slot = tmem_base + kScaleCols + s * kScaleSlot;
-                const int steps = min(4, (m.nb - 8 * kc + 1) / 2);   // 64 elements each
-                if (leader) {
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {   // slot: 4 columns of a's scales, 8 of b's, per group
-                        if (2 * g >= steps) continue;
-                        const uint32_t col = slot + g * 12;
-                        ptx::tmem_cp_scales(col, sf_hi | static_cast<uint64_t>(sf_lo + g * 32));
-                        ptx::tmem_cp_scales(col + 4, sf_hi | static_cast<uint64_t>(sf_lo + 64 + g * 32));
-                        ptx::tmem_cp_scales(col + 8, sf_hi | static_cast<uint64_t>(sf_lo + 128 + g * 32));
+                if (pipe == 0) {
+                    if (leader) {
+                        for (int g = 0; g < m.ng; ++g) ptx::tmem_cp_scales(col_a + 4 * g, sf_hi | static_cast<uint64_t>(a_sf_lo + 32 * g));
+                        ptx::umma_commit(&bar_a_scales);
                     }
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint32_t col = slot + (ks >> 1) * 12;
-                        if (ks < steps)
-                            ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
-                                           desc_hi | static_cast<uint64_t>(st + (kABytes >> 4) + ks * 2),
-                                           (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
-                    }
-                    ptx::umma_commit(&bar_empty[s]);
-                    if (kc + 1 == nkc) ptx::umma_commit(&bar_acc_full[t & 1u]);
+                    __syncwarp();
+                } else {   // (copies are in order with the products of the warp that made them only)
+                    if (!ptx::mbar_wait_warp(&bar_a_scales, seen & 1u, &abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
                 }
+                ++seen;
+                cur_qb = cur.qb;
+            }
+            const bool run_ends = RESIDENT && (i + 1 == range.count || cur.last_of_qb());
+            if ((t & 1u) == pipe) {
+                // the columns this accumulator shares with tile t - 1's (and with them all of tile t - 2's).  A barrier per
+                // accumulator: a warp that waits for every other phase of one barrier cannot tell them apart.
+                if (t && !ptx::mbar_wait_warp(&bar_shared_free[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, &abort_flag)) { ok = false; break; }
+                const uint32_t tacc = tmem_base + (t & 1u ? kAcc1 : 0u);
+                for (int kc = 0; kc < nkc; ++kc) {
+                    if (!ptx::mbar_wait_warp(&bar_full[s0 + s], ph, &abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+                    const uint32_t st = ring_lo + (s0 + s) * (kStage >> 4), sf_lo = st + (kBBytes >> 4);
+                    const uint32_t slot = col_b + (s0 + s) * scale_slot(RESIDENT);   // 8 columns of b's scales per group, then 4 of a's
+                    const uint32_t at = RESIDENT ? a_lo + kc * (kABytes >> 4) : st + ((kBBytes + kSfbBytes) >> 4);
+                    const uint32_t sa = RESIDENT ? col_a + 8 * kc : slot + 16;
+                    const int steps = min(4, (m.nb - 8 * kc + 1) / 2);   // 64 elements each
+                    if (leader) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            if (2 * g >= steps) continue;
+                            ptx::tmem_cp_scales(slot + 8 * g, sf_hi | static_cast<uint64_t>(sf_lo + g * 32));
+                            ptx::tmem_cp_scales(slot + 8 * g + 4, sf_hi | static_cast<uint64_t>(sf_lo + 64 + g * 32));
+                            if (!RESIDENT) ptx::tmem_cp_scales(sa + 4 * g, sf_hi | static_cast<uint64_t>(at + (kABytes >> 4) + g * 32));
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            if (ks < steps)
+                                ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(at + ks * 2), desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                               (ks & 1) ? kIdesc2 : kIdesc0, sa + (ks >> 1) * 4, slot + (ks >> 1) * 8, (kc | ks) ? 1u : 0u);
+                        ptx::umma_commit(&bar_empty[s0 + s]);
+                        if (kc + 1 == nkc) ptx::umma_commit(&bar_acc_full[t & 1u]);
+                    }
+                    __syncwarp();
+                    if (++s == static_cast<uint32_t>(m.half)) { s = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+            }
+            if (run_ends) {   // nothing of this query block is left on this warp
+                if (leader) ptx::umma_commit(&bar_a_free);
                 __syncwarp();
-                if (++s == kStages) { s = 0; ph ^= 1u; }
             }
         }
     } else {
-        const int quarter = warp & 3, part = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
+        const int quarter = warp & 3, part = (warp - 4) >> 2;   // TMEM lanes, columns of this warp
         const uint32_t* gnorm = static_cast<const uint32_t*>(a.bnorm);
         RowEpilogue<float, MODE, BURST, false, 2, false, !L2> epi(a);
         uint32_t t = 0;
@@ -175,8 +241,8 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             ptx::tmem_ld_wait(rb);
             ptx::tc_fence_before();
             __syncwarp();
-            // shared columns: 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
-            if (lane == 0 && (ab ? part < 2 : part >= 2)) ptx::mbar_arrive(&bar_shared_free);
+            // shared columns: 152 .. 255 of accumulator 0, 0 .. 103 of accumulator 1
+            if (lane == 0 && (ab ? part < 2 : part >= 2)) ptx::mbar_arrive(&bar_shared_free[ab]);
             if (MODE == kModeAppend && !a.direct) {
                 const uint32_t* gn = gnorm + col0;
                 if (L2) {
@@ -205,7 +271,7 @@ mx4_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 2) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, 512);
     }
@@ -219,7 +285,11 @@ cudaError_t launch_one(Mx4Args m, const CUtensorMap* mapA, const CUtensorMap* ma
     const int64_t total = static_cast<int64_t>(n_qb) * a.n_tiles_sel;
     if (total <= 0) return cudaSuccess;
     if (a.tile_step < 1) a.tile_step = 1;
-    auto kern = mx4_gemm_kernel<MODE, BURST, L2>;
+    const int chunks = (m.ng + 1) / 2;
+    const bool resident = chunks <= kResidentChunks;
+    m.half = half_stages(resident, chunks);
+    const int smem = 1024 + (resident ? chunks * (kABytes + kSfaBytes) : 0) + 2 * m.half * stage_bytes(resident);
+    auto kern = resident ? mx4_gemm_kernel<MODE, BURST, L2, true> : mx4_gemm_kernel<MODE, BURST, L2, false>;
     cudaError_t e = allow_max_smem(kern);
     if (e != cudaSuccess) return e;
     const int grid = static_cast<int>(std::min<int64_t>(total, num_sms));
@@ -232,7 +302,7 @@ cudaError_t launch_one(Mx4Args m, const CUtensorMap* mapA, const CUtensorMap* ma
     }
     const bool shared = n_qb == 1 && a.row_cands < 3LL * 4 * grid;   // (the rule of launch_dist_gemm)
     a.eager = total >= 16LL * grid && !shared ? 1 : 0;
-    kern<<<grid, kThreads, kSmemBytes, stream>>>(*mapA, *mapB, m);
+    kern<<<grid, kThreads, smem, stream>>>(*mapA, *mapB, m);
     return cudaGetLastError();
 }
 

@@ -80,7 +80,7 @@ __device__ __forceinline__ void store_one(T* o, float v) {
 
 // The end of a CTA: TMEM goes back; a split tile (bt, at), whose parts lie in shared memory as [TN][128], is added up.
 template <int THREADS, int TN, typename T>
-__device__ __forceinline__ void finish(const ProductArgs& p, int warp, uint32_t tmem_base, volatile int& abort_flag, uint8_t* smem,
+__device__ __forceinline__ void finish(const ProductArgs& p, bool owns_tmem, uint32_t tmem_base, volatile int& abort_flag, uint8_t* smem,
                                        int bt, int at, int part) {
     // After an abort, copies in flight get time to land before the shared memory is used again or released.
     __syncwarp();
@@ -90,7 +90,7 @@ __device__ __forceinline__ void finish(const ProductArgs& p, int warp, uint32_t 
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (owns_tmem) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, 512);
     }
@@ -278,31 +278,36 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         }
     }
 
-    finish<K::kThreads, TN, T>(p, warp, tmem_base, abort_flag, smem, static_cast<int>(lo / p.a_tiles), static_cast<int>(lo % p.a_tiles), part);
+    finish<K::kThreads, TN, T>(p, warp == 1, tmem_base, abort_flag, smem, static_cast<int>(lo / p.a_tiles), static_cast<int>(lo % p.a_tiles), part);
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows of a (up to 64): they and their scales stay in shared memory and in TMEM, only rows of b travel through
-// the ring, and four accumulators with an epilogue of four warps each keep four tiles on the way -- with one row of a
-// a tile is little work for anybody, and what counts is how many of the hand-offs between the roles overlap.
+// Few rows of a (up to 128): they and their scales stay in shared memory and in TMEM, and only rows of b travel through
+// the ring.  (All CTAs reading the same few rows of a again for every tile queue up at the few L2 lines that hold
+// them.)  A tile is little work for anybody, so what counts is how many of the hand-offs between the roles overlap:
+// two producers and two MMA warps take even and odd tiles, each with half of the ring, and four groups of epilogue
+// warps have four accumulators (two of 128 columns, in halves).
 // ---------------------------------------------------------------------------------------
 constexpr int kFewStage = kLanes * kChunk + 1024;
 constexpr int kFewMaxStages = 12;
-constexpr int kFewAcc = 4;
-constexpr int kFewThreads = 64 + 128 * kFewAcc;
+constexpr int kFewGroups = 4;
+constexpr int kFewThreads = 128 + 128 * kFewGroups;
 template <int TN>
-constexpr int kFewMaxChunks = TN == 64 ? 16 : 32;   // TMEM columns: accumulators, 8 a chunk of a's scales, 8 a stage
-static_assert(kFewAcc * 64 + 8 * kFewMaxChunks<64> + 8 * kFewMaxStages <= 512 && kFewAcc * 32 + 8 * kFewMaxChunks<32> + 8 * kFewMaxStages <= 512,
-              "TMEM columns");
-template <int TN>
-constexpr int few_resident_bytes(int chunks) { return chunks * (TN * kChunk + 1024); }
+struct Few {
+    static constexpr int kAcc = TN == 128 ? 2 : 4;              // accumulators
+    static constexpr int kCols = TN == 128 ? 64 : TN;           // columns of an epilogue thread
+    static constexpr int kMaxChunks = TN >= 64 ? 16 : 32;       // of a: 8 TMEM columns of scales each
+    static_assert(kAcc * TN + 8 * kMaxChunks + 8 * kFewMaxStages <= 512, "TMEM columns");
+    static constexpr int resident_bytes(int chunks) { return chunks * (TN * kChunk + 1024); }
+};
 
 template <int TN, typename T>
 __global__ void __launch_bounds__(kFewThreads, 1)
 mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
-               const __grid_constant__ ProductArgs p, const int stages) {
+               const __grid_constant__ ProductArgs p, const int half_stages) {
+    using K = Few<TN>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bar_full[kFewMaxStages], bar_empty[kFewMaxStages], bar_acc_full[kFewAcc], bar_acc_free[kFewAcc], bar_a;
+    __shared__ uint64_t bar_full[kFewMaxStages], bar_empty[kFewMaxStages], bar_acc_full[K::kAcc], bar_acc_free[K::kAcc], bar_a, bar_a_scales;
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
 
@@ -318,21 +323,22 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     uint8_t* a_scales = smem + nkc * TN * kChunk;         // [nkc][1 KB]
     uint8_t* ring = a_scales + nkc * 1024;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < 2 * half_stages; ++s) {
             ptx::mbar_init(&bar_full[s], 1);
             ptx::mbar_init(&bar_empty[s], 1);
         }
-        for (int b = 0; b < kFewAcc; ++b) {
+        for (int b = 0; b < K::kAcc; ++b) {
             ptx::mbar_init(&bar_acc_full[b], 1);
-            ptx::mbar_init(&bar_acc_free[b], 4);
+            ptx::mbar_init(&bar_acc_free[b], 4 * kFewGroups / K::kAcc);
         }
         ptx::mbar_init(&bar_a, 1);
+        ptx::mbar_init(&bar_a_scales, 1);
         abort_flag = 0;
         ptx::mbar_fence_init();
         ptx::prefetch_tensormap(&map_a);
         ptx::prefetch_tensormap(&map_b);
     }
-    if (warp == 1) {
+    if (warp == 2) {
         ptx::tmem_alloc(&tmem_base_slot, 512);
         ptx::tmem_relinquish();
     }
@@ -340,54 +346,64 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem_base = tmem_base_slot;
-    const uint32_t col_a = tmem_base + kFewAcc * TN, col_b = col_a + 8 * nkc;
+    const uint32_t col_a = tmem_base + K::kAcc * TN, col_b = col_a + 8 * nkc;
+    const uint32_t pipe = warp & 1u;                      // of producers and MMA warps
+    const uint32_t s0 = pipe * half_stages;               // first stage of this pipe's half of the ring
 
-    if (warp == 0) {
+    if (warp < 2) {
         const bool leader = ptx::elect_one();
         const uint32_t a_sf = static_cast<uint32_t>(min(p.ng, 2 * kc1) - 2 * kc0) * 512u;
-        if (leader) {
+        if (leader && pipe == 0) {
             ptx::mbar_expect_tx(&bar_a, static_cast<uint32_t>(nkc) * TN * kChunk + a_sf);
             for (int kc = kc0; kc < kc1; ++kc) ptx::tma_load_2d(a_codes + (kc - kc0) * TN * kChunk, &map_a, &bar_a, kc * kChunk, 0);
             ptx::bulk_load_1d(a_scales, p.a_scales + kc0 * 1024, a_sf, &bar_a);
         }
+        __syncwarp();
         uint32_t s = 0, ph = 0;
         bool ok = true;
-        for (int bt = lo; bt < hi && ok; ++bt) {
+        for (int bt = lo + pipe; bt < hi && ok; bt += 2) {
             const uint8_t* sb = p.b_scales + static_cast<int64_t>(bt) * p.ng * 512;
             for (int kc = kc0; kc < kc1; ++kc) {
-                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (!ptx::mbar_wait_warp(&bar_empty[s0 + s], ph ^ 1u, &abort_flag)) { ok = false; break; }
                 if (leader) {
-                    uint8_t* st = ring + s * kFewStage;
+                    uint8_t* st = ring + (s0 + s) * kFewStage;
+                    uint64_t* full = &bar_full[s0 + s];
                     const uint32_t bytes = min(2, p.ng - 2 * kc) * 512u;
-                    ptx::mbar_expect_tx(&bar_full[s], kLanes * kChunk + bytes);
-                    ptx::tma_load_2d(st, &map_b, &bar_full[s], kc * kChunk, bt * kLanes);
-                    ptx::bulk_load_1d(st + kLanes * kChunk, sb + kc * 1024, bytes, &bar_full[s]);
+                    ptx::mbar_expect_tx(full, kLanes * kChunk + bytes);
+                    ptx::tma_load_2d(st, &map_b, full, kc * kChunk, bt * kLanes);
+                    ptx::bulk_load_1d(st + kLanes * kChunk, sb + kc * 1024, bytes, full);
                 }
                 __syncwarp();
-                if (++s == static_cast<uint32_t>(stages)) { s = 0; ph ^= 1u; }
+                if (++s == static_cast<uint32_t>(half_stages)) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 1) {
+    } else if (warp < 4) {
         constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(kLanes, TN, 0), kIdesc2 = ptx::umma_idesc_mxf4(kLanes, TN, 2);
         const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
         const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
         const uint32_t a_lo = (ptx::smem_u32(a_codes) & 0x3FFFFu) >> 4, ring_lo = (ptx::smem_u32(ring) & 0x3FFFFu) >> 4;
         const uint32_t a_sf_lo = (ptx::smem_u32(a_scales) & 0x3FFFFu) >> 4;
         const bool leader = ptx::elect_one();
-        uint32_t s = 0, ph = 0, t = 0;
+        uint32_t s = 0, ph = 0, u = 0;                    // u: tiles of this pipe so far
         bool ok = ptx::mbar_wait_warp(&bar_a, 0u, &abort_flag);
-        ptx::tc_fence_after();
-        if (ok && leader)
-            for (int g = 0; g < min(p.ng, 2 * kc1) - 2 * kc0; ++g) ptx::tmem_cp_scales(col_a + 4 * g, sf_hi | static_cast<uint64_t>(a_sf_lo + 32 * g));
-        __syncwarp();
-        for (int bt = lo; bt < hi && ok; ++bt, ++t) {
-            const uint32_t ab = t % kFewAcc;
-            if (t >= kFewAcc && !ptx::mbar_wait_warp(&bar_acc_free[ab], (t / kFewAcc - 1) & 1u, &abort_flag)) { ok = false; break; }
+        if (pipe == 0) {
+            if (ok && leader) {
+                for (int g = 0; g < min(p.ng, 2 * kc1) - 2 * kc0; ++g) ptx::tmem_cp_scales(col_a + 4 * g, sf_hi | static_cast<uint64_t>(a_sf_lo + 32 * g));
+                ptx::umma_commit(&bar_a_scales);
+            }
+            __syncwarp();
+        } else if (ok) {   // (copies are in order with the products of the warp that made them only)
+            ok = ptx::mbar_wait_warp(&bar_a_scales, 0u, &abort_flag);
+            ptx::tc_fence_after();
+        }
+        for (int bt = lo + pipe; bt < hi && ok; bt += 2, ++u) {
+            const uint32_t ab = K::kAcc == 4 ? pipe + 2 * (u & 1u) : pipe, use = K::kAcc == 4 ? u >> 1 : u;   // use: of this accumulator
+            if (use && !ptx::mbar_wait_warp(&bar_acc_free[ab], (use - 1) & 1u, &abort_flag)) { ok = false; break; }
             const uint32_t tacc = tmem_base + ab * TN;
             for (int kc = kc0; kc < kc1; ++kc) {
-                if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+                if (!ptx::mbar_wait_warp(&bar_full[s0 + s], ph, &abort_flag)) { ok = false; break; }
                 ptx::tc_fence_after();
-                const uint32_t st = ring_lo + s * (kFewStage >> 4), slot = col_b + s * 8;
+                const uint32_t st = ring_lo + (s0 + s) * (kFewStage >> 4), slot = col_b + (s0 + s) * 8;
                 const uint32_t at = a_lo + (kc - kc0) * (TN * kChunk >> 4), sa = col_a + (kc - kc0) * 8;
                 const int steps = min(4, (p.nb - 8 * kc + 1) / 2);   // 64 elements each
                 if (leader) {
@@ -398,59 +414,64 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
                         if (ks < steps)
                             ptx::umma_mxf4(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2), desc_hi | static_cast<uint64_t>(at + ks * 2),
                                            (ks & 1) ? kIdesc2 : kIdesc0, slot + (ks >> 1) * 4, sa + (ks >> 1) * 4, (kc > kc0 || ks) ? 1u : 0u);
-                    ptx::umma_commit(&bar_empty[s]);
+                    ptx::umma_commit(&bar_empty[s0 + s]);
                     if (kc + 1 == kc1) ptx::umma_commit(&bar_acc_full[ab]);
                 }
                 __syncwarp();
-                if (++s == static_cast<uint32_t>(stages)) { s = 0; ph ^= 1u; }
+                if (++s == static_cast<uint32_t>(half_stages)) { s = 0; ph ^= 1u; }
             }
         }
     } else {
-        const int quarter = warp & 3, group = (warp - 2) >> 2;   // TMEM lanes; every fourth tile
+        // group g: accumulator g % kAcc, columns from (g / kAcc) * kCols on; its tiles are kAcc apart
+        const int quarter = warp & 3, group = (warp - 4) >> 2, ab = group % K::kAcc, first = group / K::kAcc * K::kCols;
         bool ok = true;
         float* parts = reinterpret_cast<float*>(smem);           // split: [TN][128]
         uint32_t turn = 0;
-        for (int bt = lo + group; bt < hi; bt += kFewAcc, ++turn) {
+        for (int bt = lo + ab; bt < hi; bt += K::kAcc, ++turn) {
             const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
-            uint32_t r[TN];
-            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[group], turn & 1u, &abort_flag);
+            uint32_t r[K::kCols];
+            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], turn & 1u, &abort_flag);
             if (ok) {
                 ptx::tc_fence_after();
-                const uint32_t tacc = tmem_base + group * TN + (static_cast<uint32_t>(quarter * 32) << 16);
-                if constexpr (TN >= 32) {
+                const uint32_t tacc = tmem_base + ab * TN + first + (static_cast<uint32_t>(quarter * 32) << 16);
+                if constexpr (K::kCols >= 32) {
 #pragma unroll
-                    for (int c = 0; c < TN; c += 32) ptx::tmem_ld_32x32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
+                    for (int c = 0; c < K::kCols; c += 32) ptx::tmem_ld_32x32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(r + c));
 #pragma unroll
-                    for (int c = 0; c < TN; c += 32) ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + c));
+                    for (int c = 0; c < K::kCols; c += 32) ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + c));
                 } else {
                     ptx::tmem_ld_32x16(tacc, r);
                     ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[16]>(r));
                 }
                 ptx::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&bar_acc_free[group]);
+                if (lane == 0) ptx::mbar_arrive(&bar_acc_free[ab]);
             } else {
                 // (as above: no numbers)
 #pragma unroll
-                for (int c = 0; c < TN; ++c) r[c] = 0x7fffffffu;
+                for (int c = 0; c < K::kCols; ++c) r[c] = 0x7fffffffu;
             }
-            if (p.split > 1) {
-                // (one tile: its commit says that every copy and product has read what lies there)
+            if (p.split > 1) {   // (one tile: its commit says that every copy and product has read what lies there)
 #pragma unroll
-                for (int c = 0; c < TN; ++c) parts[c * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
+                for (int c = 0; c < K::kCols; ++c) parts[(first + c) * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
                 continue;
             }
-            const int cols = static_cast<int>(p.m);
+            const int cols = static_cast<int>(p.m) - first;
             if (j < p.n) {
-                T* o = static_cast<T*>(p.out) + j;
+                T* o = static_cast<T*>(p.out) + first * p.ldo + j;
+                if (cols >= K::kCols) {
 #pragma unroll
-                for (int c = 0; c < TN; ++c, o += p.ldo)
-                    if (c < cols) store_one(o, __uint_as_float(r[c]));
+                    for (int c = 0; c < K::kCols; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < K::kCols; ++c, o += p.ldo)
+                        if (c < cols) store_one(o, __uint_as_float(r[c]));
+                }
             }
         }
     }
 
-    finish<kFewThreads, TN, T>(p, warp, tmem_base, abort_flag, smem, lo, 0, part);
+    finish<kFewThreads, TN, T>(p, warp == 2, tmem_base, abort_flag, smem, lo, 0, part);
 }
 
 template <int TN, typename T>
@@ -483,15 +504,15 @@ void launch(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = p.split > 1 ? 1 : 0;
-    if constexpr (TN <= 64) {
+    if constexpr (TN <= 128) {
         const int mine = (chunks + p.split - 1) / p.split;   // chunks of K of a CTA
-        const int stages = std::min(kFewMaxStages, (kSmemMost - 1024 - few_resident_bytes<TN>(mine)) / kFewStage);
-        if (mine <= kFewMaxChunks<TN> && stages >= 4) {
+        const int half = std::min(kFewMaxStages, (kSmemMost - 1024 - Few<TN>::resident_bytes(mine)) / kFewStage) / 2;
+        if (mine <= Few<TN>::kMaxChunks && half >= 3) {   // (64 x 16 384 x 4096 with four stages: 15.7 us; through the ring 12.2)
             auto kern = mx4_few_kernel<TN, T>;
             B200_CUDA_CHECK(allow_max_smem(kern));
             cfg.blockDim = dim3(kFewThreads);
-            cfg.dynamicSmemBytes = 1024 + few_resident_bytes<TN>(mine) + stages * kFewStage;
-            B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p, stages));
+            cfg.dynamicSmemBytes = 1024 + Few<TN>::resident_bytes(mine) + 2 * half * kFewStage;
+            B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p, half));
             return;
         }
     }
