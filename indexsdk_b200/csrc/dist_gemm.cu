@@ -707,8 +707,10 @@ int encode_operand_map(CUtensorMap* out, int kind, const void* base, int64_t row
     return encode_rows_map(out, dt, elem, base, rows, d, box_rows);
 }
 
-int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int cols,
-                    int box_rows) {
+namespace {
+
+int encode_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int cols, int box_cols,
+               int box_rows, CUtensorMapSwizzle swizzle) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -723,12 +725,22 @@ int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const 
     }
     cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     cuuint64_t gstride[1] = {static_cast<cuuint64_t>(cols) * elem};
-    cuuint32_t box[2] = {static_cast<cuuint32_t>(kChunkBytes / elem), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estride[2] = {1, 1};
     CUresult r = encode(out, type, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
+}
+
+}  // namespace
+
+int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int cols,
+                    int box_rows) {
+    return encode_map(out, type, elem, base, rows, cols, kChunkBytes / elem, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int encode_plain_map(CUtensorMap* out, const void* base, int64_t rows, int words, int box_rows) {
+    return encode_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, base, rows, words, words, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace b200

@@ -523,13 +523,237 @@ void launch(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
     B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p));
 }
 
+// ---------------------------------------------------------------------------------------
+// Many rows of both: a pair of CTAs makes 256 x 256 tiles, 128 rows of b each, and each loads only half of a's rows --
+// 32 KB of codes per 256 elements of K instead of 48, which is what a single CTA's ring waits for.  CTA 0 issues for
+// both; its barriers count both CTAs' copies, and its commits arrive in both.  TMEM as above, five stages of 24 columns
+// of scales: the accumulators share 120 columns (0-255 and 136-391).
+// ---------------------------------------------------------------------------------------
+constexpr int kPairStages = 5;
+constexpr int kPairHalf = 128 * kChunk;                                   // 16 KB: this CTA's rows of b, or of a
+constexpr int kPairStage = 2 * kPairHalf + 3 * 1024;                      // and scales: b's own 128 rows, all 256 of a
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+constexpr int kPairThreads = 64 + 32 * 16;
+constexpr uint32_t kPairAcc1 = 136, kPairScaleCol = 392;
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+                const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_sa,
+                const __grid_constant__ ProductArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[kPairStages], bar_empty[kPairStages], bar_acc_full[2], bar_acc_free;
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_rank();
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int chunks = (p.ng + 1) / 2;
+    const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;     // b_tiles: of 256 rows
+    const int workers = gridDim.x / 2, worker = blockIdx.x / 2;
+    const int64_t lo = total * worker / workers, hi = total * (worker + 1) / workers;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            ptx::mbar_init(&bar_full[s], 1);
+            ptx::mbar_init(&bar_empty[s], 1);
+        }
+        ptx::mbar_init(&bar_acc_full[0], 1);
+        ptx::mbar_init(&bar_acc_full[1], 1);
+        ptx::mbar_init(&bar_acc_free, 16);   // CTA 0's: eight warps of each CTA
+        abort_flag = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&map_a);
+        ptx::prefetch_tensormap(&map_b);
+        ptx::prefetch_tensormap(&map_sa);
+        ptx::prefetch_tensormap(&map_sb);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(&tmem_base_slot, 512);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();   // (the other CTA's barriers exist)
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+
+    if (warp == 0) {
+        const bool leader = ptx::elect_one();
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        int bt = static_cast<int>(lo / p.a_tiles), at = static_cast<int>(lo % p.a_tiles);
+        for (int64_t i = lo; i < hi && ok; ++i, next_tile(p, bt, at)) {
+            for (int kc = 0; kc < chunks; ++kc) {
+                if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
+                if (leader) {
+                    uint8_t* st = smem + s * kPairStage;
+                    uint8_t* sf = st + 2 * kPairHalf;
+                    const uint32_t full = ptx::cluster_addr(ptx::smem_u32(&bar_full[s]), 0);
+                    if (rank == 0) ptx::mbar_expect_tx(&bar_full[s], 2 * kPairStage);
+                    ptx::tma_load_2d_pair(st, &map_b, full, kc * kChunk, bt * 256 + static_cast<int>(rank) * 128);
+                    ptx::tma_load_2d_pair(st + kPairHalf, &map_a, full, kc * kChunk, at * 256 + static_cast<int>(rank) * 128);
+                    // (two groups; behind a row's last group the next 128 rows' first, which nobody uses, or zeros)
+                    ptx::tma_load_2d_pair(sf, &map_sb, full, 0, (bt * 2 + static_cast<int>(rank)) * p.ng + 2 * kc);
+                    ptx::tma_load_2d_pair(sf + 1024, &map_sa, full, 0, at * 2 * p.ng + 2 * kc);
+                    ptx::tma_load_2d_pair(sf + 2048, &map_sa, full, 0, (at * 2 + 1) * p.ng + 2 * kc);
+                }
+                __syncwarp();
+                if (++s == kPairStages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            constexpr uint32_t kIdesc0 = ptx::umma_idesc_mxf4(256, 256, 0), kIdesc2 = ptx::umma_idesc_mxf4(256, 256, 2);
+            const uint64_t desc_hi = ptx::umma_desc_k_sw128(0);
+            const uint64_t sf_hi = ptx::umma_desc_k_plain(0, 128u, 128u);
+            const uint32_t ring_lo = (ptx::smem_u32(smem) & 0x3FFFFu) >> 4;
+            const bool leader = ptx::elect_one();
+            uint32_t s = 0, ph = 0, t = 0;
+            bool ok = true;
+            for (int64_t i = lo; i < hi && ok; ++i, ++t) {
+                // both CTAs have tile t - 1's shared columns in registers (and with them all of tile t - 2)
+                if (t && !ptx::mbar_wait_warp_cluster(&bar_acc_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + (t & 1u ? kPairAcc1 : 0u);
+                for (int kc = 0; kc < chunks; ++kc) {
+                    if (!ptx::mbar_wait_warp(&bar_full[s], ph, &abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+                    const uint32_t st = ring_lo + s * (kPairStage >> 4), sf_lo = st + (2 * kPairHalf >> 4);
+                    const uint32_t slot = tmem_base + kPairScaleCol + s * 24;
+                    const int steps = min(4, (p.nb - 8 * kc + 1) / 2);   // 64 elements each
+                    if (leader) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+                            if (2 * g < steps)
+#pragma unroll
+                                for (int h = 0; h < 3; ++h)
+                                    ptx::tmem_cp_scales_pair(slot + g * 12 + 4 * h, sf_hi | static_cast<uint64_t>(sf_lo + 64 * h + 32 * g));
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t col = slot + (ks >> 1) * 12;
+                            if (ks < steps)
+                                ptx::umma_mxf4_pair(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                                    desc_hi | static_cast<uint64_t>(st + (kPairHalf >> 4) + ks * 2),
+                                                    (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
+                        }
+                        ptx::umma_commit_pair(&bar_empty[s]);
+                        if (kc + 1 == chunks) ptx::umma_commit_pair(&bar_acc_full[t & 1u]);
+                    }
+                    __syncwarp();
+                    if (++s == kPairStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, group = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
+        const uint32_t free_at = ptx::cluster_addr(ptx::smem_u32(&bar_acc_free), 0);
+        uint32_t t = 0;
+        bool ok = true;
+        int bt = static_cast<int>(lo / p.a_tiles), at = static_cast<int>(lo % p.a_tiles);
+        for (int64_t i = lo; i < hi; ++i, ++t, next_tile(p, bt, at)) {
+            const int64_t j = static_cast<int64_t>(bt) * 256 + rank * 128 + quarter * 32 + lane;
+            const int64_t i0 = static_cast<int64_t>(at) * 256 + group * 64;
+            const uint32_t ab = t & 1u;
+            uint32_t r[64];
+            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
+            if (ok) {
+                ptx::tc_fence_after();
+                const uint32_t tacc = tmem_base + (ab ? kPairAcc1 : 0u) + group * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
+                ptx::tmem_ld_32x32(tacc, *reinterpret_cast<uint32_t(*)[32]>(r));
+                ptx::tmem_ld_32x32(tacc + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+                ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r));
+                ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
+                ptx::tc_fence_before();
+                __syncwarp();
+                // shared: 136 .. 255 of accumulator 0, 0 .. 119 of accumulator 1
+                if (lane == 0 && (ab ? group < 2 : group >= 2)) ptx::mbar_arrive_cluster(free_at);
+            } else {
+                // (as above: no numbers)
+#pragma unroll
+                for (int c = 0; c < 64; ++c) r[c] = 0x7fffffffu;
+            }
+            const int cols = static_cast<int>(min(p.m - i0, static_cast<int64_t>(64)));
+            if (j < p.n) {
+                T* o = static_cast<T*>(p.out) + i0 * p.ldo + j;
+                if (cols >= 64) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c, o += p.ldo)
+                        if (c < cols) store_one(o, __uint_as_float(r[c]));
+                }
+            }
+        }
+    }
+
+    // (after an abort, copies in flight get time to land; neither CTA's memory goes before both are done)
+    __syncwarp();
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) { }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <typename T>
+bool launch_pair(const Mx4ProductArgs& q, cudaStream_t st) {
+    auto kern = mx4_pair_kernel<T>;
+    B200_CUDA_CHECK(allow_max_smem(kern));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // pairs that the device runs at a time (an odd number of SMs in a group leaves one without a partner)
+    static const int pairs = [&] {
+        int v = 0;
+        cfg.gridDim = dim3(2);
+        return cudaOccupancyMaxActiveClusters(&v, kern, &cfg) == cudaSuccess ? v : 0;
+    }();
+    ProductArgs p{};
+    p.a_scales = q.a_scales;
+    p.b_scales = q.b_scales;
+    p.nb = mx4_blocks(q.d);
+    p.ng = mx4_groups(q.d);
+    p.m = q.m;
+    p.n = q.n;
+    p.out = q.out;
+    p.ldo = q.ldo;
+    p.split = 1;
+    p.a_tiles = div_up(q.m, 256);
+    p.b_tiles = div_up(q.n, 256);
+    const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;
+    if (pairs <= 0 || total < pairs) return false;
+    CUtensorMap map_a, map_b, map_sa, map_sb;
+    const int64_t rows_a = (q.m + 127) / 128 * p.ng, rows_b = (q.n + 127) / 128 * p.ng;
+    if (encode_mx4_map(&map_a, q.a_codes, q.m, q.d, 128) != 0 || encode_mx4_map(&map_b, q.b_codes, q.n, q.d, 128) != 0 ||
+        encode_plain_map(&map_sa, q.a_scales, rows_a, 128, 2) != 0 || encode_plain_map(&map_sb, q.b_scales, rows_b, 128, 2) != 0)
+        throw std::runtime_error("cuTensorMapEncodeTiled failed for the rows of a product");
+    cfg.gridDim = dim3(2 * static_cast<unsigned>(pairs));
+    B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, map_sb, map_sa, p));
+    return true;
+}
+
 template <typename T>
 void product(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
     if (q.m <= 16) launch<16, T>(q, num_sms, st);
     else if (q.m <= 32) launch<32, T>(q, num_sms, st);
     else if (q.m <= 64) launch<64, T>(q, num_sms, st);
     else if (q.m <= 128) launch<128, T>(q, num_sms, st);
-    else launch<256, T>(q, num_sms, st);
+    else if (!launch_pair<T>(q, st)) launch<256, T>(q, num_sms, st);
 }
 
 }  // namespace

@@ -107,8 +107,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // loads stay coalesced).  The next row's loads are on their way while this one is reduced and written.
 //
 // A rounding to whole numbers shows every error of its argument where that lies next to a border, and for 16-bit
-// rows with weights of 16 bits one element in 20 000 lies exactly ON a border.  So squares are added up in fp32 over
-// eight elements only, fp32 rows keep what the largest product loses to its rounding, and an element whose fp32
+// rows with weights of 16 bits one element in 20 000 lies exactly ON a border.  So squares are added up in
+// 64 bits (with a scale per row over eight elements in fp32 first), fp32 rows keep their largest product unrounded, and an element whose fp32
 // quotient is within 2^-14 of a border (that quotient is off by at most 127 * 6 * 2^-24) is compared with it in 64 bits.
 // ---------------------------------------------------------------------------------------
 template <int NT>
@@ -283,7 +283,12 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
                     top_w = w[e];
                 }
             }
-            ssq += part;
+            if (a.static_scale) {   // (nothing cancels an error of the sum there)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ssq = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ssq);
+            } else {
+                ssq += part;
+            }
             if (!kLow) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) top = max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));

@@ -246,7 +246,8 @@ def random_operand(rng, n, d, spread=2, fill=127):
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("m, n, d", [(1, 1, 1), (1, 64, 32), (2, 300, 64), (3, 257, 33), (17, 1000, 128), (64, 129, 160),
                                      (65, 511, 256), (127, 256, 288), (128, 257, 1000), (129, 300, 96), (200, 70, 544),
-                                     (1, 5000, 768), (16, 4096, 2048), (5, 130, 4096), (300, 600, 4100), (2, 40, 16384)])
+                                     (1, 5000, 768), (16, 4096, 2048), (5, 130, 4096), (300, 600, 4100), (2, 40, 16384),
+                                     (2100, 2300, 96), (700, 7000, 544), (2049, 2305, 4100), (4000, 1300, 33)])
 def test_mx4_product(b200, m, n, d, dtype):
     """Sums that fp32 holds exactly: products are quarters times at least 2^-4, sums stay below 2^24 of those
     (|sum| <= 36 d 2^2, in steps of 2^-6: d <= 2^24 / (36 * 2^8) = 1820; longer rows use equal scales:
