@@ -709,8 +709,9 @@ int encode_operand_map(CUtensorMap* out, int kind, const void* base, int64_t row
 
 namespace {
 
-int encode_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int cols, int box_cols,
-               int box_rows, CUtensorMapSwizzle swizzle) {
+// dims, box: ndim extents in elements, innermost first; rows without gaps
+int encode_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int ndim, const cuuint64_t* dims,
+               const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -723,12 +724,10 @@ int encode_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void*
             return -1;
         encode = reinterpret_cast<EncodeFn>(fn);
     }
-    cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-    cuuint64_t gstride[1] = {static_cast<cuuint64_t>(cols) * elem};
-    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estride[2] = {1, 1};
-    CUresult r = encode(out, type, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint64_t stride[2] = {dims[0] * elem, ndim > 2 ? dims[0] * dims[1] * elem : 0};
+    cuuint32_t estride[3] = {1, 1, 1};
+    CUresult r = encode(out, type, static_cast<cuuint32_t>(ndim), const_cast<void*>(base), dims, stride, box, estride,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
 }
 
@@ -736,11 +735,15 @@ int encode_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void*
 
 int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int cols,
                     int box_rows) {
-    return encode_map(out, type, elem, base, rows, cols, kChunkBytes / elem, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(kChunkBytes / elem), static_cast<cuuint32_t>(box_rows)};
+    return encode_map(out, type, elem, base, 2, dims, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int encode_plain_map(CUtensorMap* out, const void* base, int64_t rows, int words, int box_rows) {
-    return encode_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, base, rows, words, words, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
+int encode_scale_map(CUtensorMap* out, const void* base, int64_t granules, int groups, int box_granules) {
+    const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(groups), static_cast<cuuint64_t>(granules)};
+    const cuuint32_t box[3] = {128, 2, static_cast<cuuint32_t>(box_granules)};
+    return encode_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, base, 3, dims, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace b200

@@ -135,7 +135,8 @@ int encode_operand_map(CUtensorMap* out, int kind, const void* base, int64_t row
 // The same for any row-major array: rows of `cols` elements of elem_bytes each.
 int encode_rows_map(CUtensorMap* out, CUtensorMapDataType type, int elem_bytes, const void* base, int64_t rows, int cols,
                     int box_rows);
-// Rows of `words` 32-bit words, boxes of box_rows whole rows, no swizzle.
-int encode_plain_map(CUtensorMap* out, const void* base, int64_t rows, int words, int box_rows);
+// Scales of microscaled 4-bit rows: blocks of 512 bytes, `groups` for every 128 rows; boxes of two groups of `box_granules`
+// times 128 rows, no swizzle.
+int encode_scale_map(CUtensorMap* out, const void* base, int64_t granules, int groups, int box_granules);
 
 }  // namespace b200

@@ -78,6 +78,21 @@ __device__ __forceinline__ void store_one(T* o, float v) {
     else *o = __float2bfloat16_rn(v);
 }
 
+// COLS accumulator columns (rows of a) of this lane's output column j -> out; `cols` of them exist.
+template <int COLS, typename T>
+__device__ __forceinline__ void store_columns(const uint32_t (&r)[COLS], const ProductArgs& p, int64_t i0, int64_t j, int cols) {
+    T* o = static_cast<T*>(p.out) + i0 * p.ldo + j;
+    if (j >= p.n) return;
+    if (cols >= COLS) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
+    } else {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c, o += p.ldo)
+            if (c < cols) store_one(o, __uint_as_float(r[c]));
+    }
+}
+
 // The end of a CTA: TMEM goes back; a split tile (bt, at), whose parts lie in shared memory as [TN][128], is added up.
 template <int THREADS, int TN, typename T>
 __device__ __forceinline__ void finish(const ProductArgs& p, bool owns_tmem, uint32_t tmem_base, volatile int& abort_flag, uint8_t* smem,
@@ -263,18 +278,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 for (int c = 0; c < K::kCols; ++c) parts[(group * K::kCols + c) * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
                 continue;
             }
-            const int cols = static_cast<int>(min(p.m - i0, static_cast<int64_t>(K::kCols)));
-            if (j < p.n) {
-                T* o = static_cast<T*>(p.out) + i0 * p.ldo + j;
-                if (cols >= K::kCols) {
-#pragma unroll
-                    for (int c = 0; c < K::kCols; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < K::kCols; ++c, o += p.ldo)
-                        if (c < cols) store_one(o, __uint_as_float(r[c]));
-                }
-            }
+            store_columns<K::kCols, T>(r, p, i0, j, static_cast<int>(min(p.m - i0, static_cast<int64_t>(K::kCols))));
         }
     }
 
@@ -456,18 +460,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
                 for (int c = 0; c < K::kCols; ++c) parts[(first + c) * kLanes + quarter * 32 + lane] = __uint_as_float(r[c]);
                 continue;
             }
-            const int cols = static_cast<int>(p.m) - first;
-            if (j < p.n) {
-                T* o = static_cast<T*>(p.out) + first * p.ldo + j;
-                if (cols >= K::kCols) {
-#pragma unroll
-                    for (int c = 0; c < K::kCols; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < K::kCols; ++c, o += p.ldo)
-                        if (c < cols) store_one(o, __uint_as_float(r[c]));
-                }
-            }
+            store_columns<K::kCols, T>(r, p, first, j, static_cast<int>(p.m) - first);
         }
     }
 
@@ -526,15 +519,15 @@ void launch(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------
 // Many rows of both: a pair of CTAs makes 256 x 256 tiles, 128 rows of b each, and each loads only half of a's rows --
 // 32 KB of codes per 256 elements of K instead of 48, which is what a single CTA's ring waits for.  CTA 0 issues for
-// both; its barriers count both CTAs' copies, and its commits arrive in both.  TMEM as above, five stages of 24 columns
-// of scales: the accumulators share 120 columns (0-255 and 136-391).
+// both; its barriers count both CTAs' copies, and its commits arrive in both.  TMEM as above, six stages of 24 columns
+// of scales: the accumulators share 144 columns (0-255 and 112-367).
 // ---------------------------------------------------------------------------------------
-constexpr int kPairStages = 5;
+constexpr int kPairStages = 6;
 constexpr int kPairHalf = 128 * kChunk;                                   // 16 KB: this CTA's rows of b, or of a
 constexpr int kPairStage = 2 * kPairHalf + 3 * 1024;                      // and scales: b's own 128 rows, all 256 of a
 constexpr int kPairSmem = kPairStages * kPairStage + 1024;
-constexpr int kPairThreads = 64 + 32 * 16;
-constexpr uint32_t kPairAcc1 = 136, kPairScaleCol = 392;
+constexpr int kPairThreads = 128 + 32 * 16;
+constexpr uint32_t kPairAcc1 = 112, kPairScaleCol = 368;
 
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
@@ -560,7 +553,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
         }
         ptx::mbar_init(&bar_acc_full[0], 1);
         ptx::mbar_init(&bar_acc_full[1], 1);
-        ptx::mbar_init(&bar_acc_free, 16);   // CTA 0's: eight warps of each CTA
+        ptx::mbar_init(&bar_acc_free, 24);   // CTA 0's: twelve warps of each CTA
         abort_flag = 0;
         ptx::mbar_fence_init();
         ptx::prefetch_tensormap(&map_a);
@@ -578,7 +571,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     ptx::tc_fence_after();
     const uint32_t tmem_base = tmem_base_slot;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {   // codes; scales
         const bool leader = ptx::elect_one();
         uint32_t s = 0, ph = 0;
         bool ok = true;
@@ -588,15 +581,15 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
                 if (!ptx::mbar_wait_warp(&bar_empty[s], ph ^ 1u, &abort_flag)) { ok = false; break; }
                 if (leader) {
                     uint8_t* st = smem + s * kPairStage;
-                    uint8_t* sf = st + 2 * kPairHalf;
                     const uint32_t full = ptx::cluster_addr(ptx::smem_u32(&bar_full[s]), 0);
-                    if (rank == 0) ptx::mbar_expect_tx(&bar_full[s], 2 * kPairStage);
-                    ptx::tma_load_2d_pair(st, &map_b, full, kc * kChunk, bt * 256 + static_cast<int>(rank) * 128);
-                    ptx::tma_load_2d_pair(st + kPairHalf, &map_a, full, kc * kChunk, at * 256 + static_cast<int>(rank) * 128);
-                    // (two groups; behind a row's last group the next 128 rows' first, which nobody uses, or zeros)
-                    ptx::tma_load_2d_pair(sf, &map_sb, full, 0, (bt * 2 + static_cast<int>(rank)) * p.ng + 2 * kc);
-                    ptx::tma_load_2d_pair(sf + 1024, &map_sa, full, 0, at * 2 * p.ng + 2 * kc);
-                    ptx::tma_load_2d_pair(sf + 2048, &map_sa, full, 0, (at * 2 + 1) * p.ng + 2 * kc);
+                    if (warp == 0) {
+                        if (rank == 0) ptx::mbar_expect_tx(&bar_full[s], 2 * kPairStage);
+                        ptx::tma_load_2d_pair(st, &map_b, full, kc * kChunk, bt * 256 + static_cast<int>(rank) * 128);
+                        ptx::tma_load_2d_pair(st + kPairHalf, &map_a, full, kc * kChunk, at * 256 + static_cast<int>(rank) * 128);
+                    } else {   // two groups of 128 rows; zeros behind a row's last group and behind the last rows
+                        ptx::tma_load_3d_pair(st + 2 * kPairHalf, &map_sb, full, 0, 2 * kc, bt * 2 + static_cast<int>(rank));
+                        ptx::tma_load_3d_pair(st + 2 * kPairHalf + 1024, &map_sa, full, 0, 2 * kc, at * 2);
+                    }
                 }
                 __syncwarp();
                 if (++s == kPairStages) { s = 0; ph ^= 1u; }
@@ -613,7 +606,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
             bool ok = true;
             for (int64_t i = lo; i < hi && ok; ++i, ++t) {
                 // both CTAs have tile t - 1's shared columns in registers (and with them all of tile t - 2)
-                if (t && !ptx::mbar_wait_warp_cluster(&bar_acc_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
+                if (t && !ptx::mbar_wait_warp(&bar_acc_free, (t - 1u) & 1u, &abort_flag)) { ok = false; break; }
                 ptx::tc_fence_after();
                 const uint32_t tacc = tmem_base + (t & 1u ? kPairAcc1 : 0u);
                 for (int kc = 0; kc < chunks; ++kc) {
@@ -645,8 +638,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
                 }
             }
         }
-    } else {
-        const int quarter = warp & 3, group = (warp - 2) >> 2;   // TMEM lanes, columns of this warp
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, group = (warp - 4) >> 2;   // TMEM lanes, columns of this warp
         const uint32_t free_at = ptx::cluster_addr(ptx::smem_u32(&bar_acc_free), 0);
         uint32_t t = 0;
         bool ok = true;
@@ -666,25 +659,14 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
                 ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
                 ptx::tc_fence_before();
                 __syncwarp();
-                // shared: 136 .. 255 of accumulator 0, 0 .. 119 of accumulator 1
-                if (lane == 0 && (ab ? group < 2 : group >= 2)) ptx::mbar_arrive_cluster(free_at);
+                // shared: 112 .. 255 of accumulator 0, 0 .. 143 of accumulator 1
+                if (lane == 0 && (ab ? group < 3 : group >= 1)) ptx::mbar_arrive_cluster(free_at);
             } else {
                 // (as above: no numbers)
 #pragma unroll
                 for (int c = 0; c < 64; ++c) r[c] = 0x7fffffffu;
             }
-            const int cols = static_cast<int>(min(p.m - i0, static_cast<int64_t>(64)));
-            if (j < p.n) {
-                T* o = static_cast<T*>(p.out) + i0 * p.ldo + j;
-                if (cols >= 64) {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c, o += p.ldo) store_one(o, __uint_as_float(r[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c, o += p.ldo)
-                        if (c < cols) store_one(o, __uint_as_float(r[c]));
-                }
-            }
+            store_columns<64, T>(r, p, i0, j, static_cast<int>(min(p.m - i0, static_cast<int64_t>(64))));
         }
     }
 
@@ -738,9 +720,9 @@ bool launch_pair(const Mx4ProductArgs& q, cudaStream_t st) {
     const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;
     if (pairs <= 0 || total < pairs) return false;
     CUtensorMap map_a, map_b, map_sa, map_sb;
-    const int64_t rows_a = (q.m + 127) / 128 * p.ng, rows_b = (q.n + 127) / 128 * p.ng;
     if (encode_mx4_map(&map_a, q.a_codes, q.m, q.d, 128) != 0 || encode_mx4_map(&map_b, q.b_codes, q.n, q.d, 128) != 0 ||
-        encode_plain_map(&map_sa, q.a_scales, rows_a, 128, 2) != 0 || encode_plain_map(&map_sb, q.b_scales, rows_b, 128, 2) != 0)
+        encode_scale_map(&map_sa, q.a_scales, (q.m + 127) / 128, p.ng, 2) != 0 ||
+        encode_scale_map(&map_sb, q.b_scales, (q.n + 127) / 128, p.ng, 1) != 0)
         throw std::runtime_error("cuTensorMapEncodeTiled failed for the rows of a product");
     cfg.gridDim = dim3(2 * static_cast<unsigned>(pairs));
     B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, map_b, map_a, map_sb, map_sa, p));

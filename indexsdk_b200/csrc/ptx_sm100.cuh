@@ -119,15 +119,11 @@ __device__ __forceinline__ float cluster_load(uint32_t cluster_address) {
     return v;
 }
 
-// Arrival at a barrier of another CTA of the cluster (address from cluster_addr), and the wait that sees what
-// such arrivals release.
+// Arrival at a barrier of another CTA of the cluster (address from cluster_addr), for what the other side reads or
+// overwrites in TMEM only: it does not wait for this thread's stores to memory, which a release would (1 700 cycles
+// behind an epilogue's).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_address) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
-}
-__device__ __forceinline__ bool mbar_wait_warp_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (!mbar_wait_warp(bar, parity, abort_flag)) return false;
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    return true;
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
 }
 
 // ---- TMA ----
@@ -151,6 +147,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_address), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster_address, int32_t x,
+                                                 int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_address), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
