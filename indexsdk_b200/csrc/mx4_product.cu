@@ -251,7 +251,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
             const int64_t i0 = static_cast<int64_t>(at) * TN + group * K::kCols;
             const uint32_t ab = t & 1u;
             uint32_t r[K::kCols];
-            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
+            if (ok) ok = ptx::mbar_wait_warp(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
             if (ok) {
                 ptx::tc_fence_after();
                 const uint32_t tacc = tmem_base + (ab ? K::kAcc1 : 0u) + group * K::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -434,7 +434,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
         for (int bt = lo + ab; bt < hi; bt += K::kAcc, ++turn) {
             const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
             uint32_t r[K::kCols];
-            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], turn & 1u, &abort_flag);
+            if (ok) ok = ptx::mbar_wait_warp(&bar_acc_full[ab], turn & 1u, &abort_flag);
             if (ok) {
                 ptx::tc_fence_after();
                 const uint32_t tacc = tmem_base + ab * TN + first + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -649,7 +649,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
             const int64_t i0 = static_cast<int64_t>(at) * 256 + group * 64;
             const uint32_t ab = t & 1u;
             uint32_t r[64];
-            if (ok) ok = ptx::mbar_wait_bounded(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
+            if (ok) ok = ptx::mbar_wait_warp(&bar_acc_full[ab], (t >> 1) & 1u, &abort_flag);
             if (ok) {
                 ptx::tc_fence_after();
                 const uint32_t tacc = tmem_base + (ab ? kPairAcc1 : 0u) + group * 64 + (static_cast<uint32_t>(quarter * 32) << 16);

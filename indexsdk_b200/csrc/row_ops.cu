@@ -1,4 +1,5 @@
 #include "row_ops.cuh"
+#include "ptx_sm100.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -90,12 +91,6 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
     Row8<T> k;
     pack8<T>(f, k);
     store8<T>(p, k);
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -291,7 +286,7 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             }
             if (!kLow) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) top = max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
+                for (int e = 0; e < 8; e += 2) top = ptx::max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
             }
         }
         if (kAhead && row + step < a.n) fetch_row(row + step);
@@ -342,7 +337,7 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
                 const float r0 = fmaf(v[j][e], c, 12582912.f), r1 = fmaf(v[j][e + 1], c, 12582912.f);
                 b[e] = __float_as_uint(r0);
                 b[e + 1] = __float_as_uint(r1);
-                off = max3(off, fabsf(fmaf(v[j][e], c, 12582912.f - r0)), fabsf(fmaf(v[j][e + 1], c, 12582912.f - r1)));
+                off = ptx::max3(off, fabsf(fmaf(v[j][e], c, 12582912.f - r0)), fabsf(fmaf(v[j][e + 1], c, 12582912.f - r1)));
             }
             if (off > 0.5f - 1.f / 16384.f) near |= 1u << j;
             uint2 o;
