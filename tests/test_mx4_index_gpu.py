@@ -50,7 +50,8 @@ def data(seed, n, nq, d):
 @pytest.mark.parametrize("metric", [0, 1])
 @pytest.mark.parametrize("n, nq, d, k", [(1, 1, 16, 1), (5, 3, 32, 8), (255, 1, 48, 10), (257, 130, 128, 5), (1000, 7, 256, 100),
                                          (20000, 1, 128, 10), (30000, 129, 64, 10), (3000, 20, 1024, 50), (700, 3, 4096, 20),
-                                         (70000, 33, 96, 1), (9000, 5, 272, 1000), (200000, 65, 128, 100)])
+                                         (70000, 33, 96, 1), (9000, 5, 272, 1000), (200000, 65, 128, 100),
+                                         (3000, 260, 2048, 10), (66000, 300, 512, 7), (40000, 1, 1040, 3)])
 def test_search(b200, n, nq, d, k, metric):
     x, q = data(n + d, n, nq, d)
     ix = b200.IndexFlat(d, metric, b200.MX4)

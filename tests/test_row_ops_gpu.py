@@ -97,7 +97,8 @@ def test_mx4_quantize_borders_and_special_values(b200):
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("n, d, ld", [(1, 1, 0), (3, 33, 0), (130, 128, 0), (7, 777, 780), (5, 100, 101), (2, 4096, 0)])
+@pytest.mark.parametrize("n, d, ld", [(1, 1, 0), (9, 5, 0), (3, 33, 0), (130, 128, 0), (7, 777, 780), (5, 100, 101), (2, 4096, 0),
+                                      (300, 777, 0), (6, 96, 104), (40, 9, 0)])
 def test_mx4_dequantize(b200, n, d, ld, dtype):
     rng = np.random.default_rng(d)
     rc, rs = ref.random_mx4(rng, n, d, spread=9)
@@ -178,10 +179,11 @@ def test_rms_norm_strides(b200, ld, offset, ldq, dtype):
 
 
 @pytest.mark.parametrize("place", ["x", "residual"])
-@pytest.mark.parametrize("d", [64, 77, 4096])
-def test_rms_norm_sum_in_place(b200, place, d):
+@pytest.mark.parametrize("n, d, dtype", [(5, 64, 2), (5, 77, 2), (5, 4096, 2), (20000, 64, 2), (15001, 77, 1), (3000, 1024, 0), (1500, 4096, 2)])
+def test_rms_norm_sum_in_place(b200, place, n, d, dtype):
+    """(With many rows a thread's next row is on its way while it writes this one.)"""
     rng = np.random.default_rng(4)
-    x, r, w = _rows(rng, 5, d, 2), _rows(rng, 5, d, 2), _rows(rng, 1, d, 2).view(-1)
+    x, r, w = _rows(rng, n, d, dtype), _rows(rng, n, d, dtype), _rows(rng, 1, d, dtype).view(-1)
     x0, r0 = x.clone(), r.clone()
     q, scales, total = rms(b200, x, w, residual=r, in_place=place)
     check_rms(x0, w, 1e-6, q, scales, total, r0)
@@ -207,6 +209,44 @@ def test_rms_norm_range(b200):
     for s in (0.0, -1.0, float("nan"), float("inf")):
         q, _, _ = rms(b200, x, w, static=torch.tensor([s], device="cuda"))
         assert bool((q == 0).all())
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("d, dtype", [(20, 0), (100, 1), (100, 2), (128, 0), (250, 2), (500, 1), (900, 2)])
+def test_rms_norm_range_next_to_others(b200, d, dtype, residual):
+    """Rows that leave the fast path between rows that do not, in one warp and in one block."""
+    rng = np.random.default_rng(10)
+    n = 700
+    base = rng.standard_normal((n, d))
+    huge, tiny = (3e4, 1e-6) if dtype == 1 else (1e36, 1e-33)
+    kind = rng.integers(0, 8, n)
+    base[kind == 0] *= huge / np.abs(base).max()
+    base[kind == 1] *= tiny
+    base[kind == 2] = 0
+    x = torch.from_numpy(base).to("cuda", ref.TORCH[dtype])
+    bad = torch.from_numpy((kind == 3) | (kind == 4)).cuda()
+    x[torch.from_numpy(kind == 3).cuda(), d // 2] = float("nan")
+    x[torch.from_numpy(kind == 4).cuda(), 0] = float("inf")
+    w = _rows(rng, 1, d, dtype, 0.1).view(-1)
+    r = torch.zeros_like(x) if residual else None
+    q, scales, total = rms(b200, x, w, residual=r)
+    assert bool(torch.isnan(scales[bad]).all()) and bool((q[bad] == 0).all())
+    if dtype == 1:   # (fp16 rows of subnormal numbers: their values are exact, as every fp16 value is in 64 bits)
+        assert float(x[torch.from_numpy(kind == 1).cuda()].abs().max()) < 1e-4
+    good = ~bad
+    check_rms(x[good], w, 1e-6, q[good], scales[good], None if total is None else total[good], None if r is None else r[good])
+
+
+def test_rms_norm_ties(b200):
+    """Products that lie exactly between two steps go to the even one: s w 254 / max is a whole odd number."""
+    d = 64
+    rng = np.random.default_rng(12)
+    x = rng.integers(-254, 255, (500, d)).astype(np.float64)
+    x[:, 0] = 254          # scale 2 after the norm's factor: every odd number is half way
+    for dtype in (0, 1):   # (bf16 holds only some of these numbers)
+        xt = torch.from_numpy(x).to("cuda", ref.TORCH[dtype])
+        q, _, _ = rms(b200, xt, torch.ones(d, dtype=ref.TORCH[dtype], device="cuda"))
+        np.testing.assert_array_equal(q.cpu().numpy(), np.rint(x / 2))   # (numpy rounds halves to even)
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
@@ -314,6 +354,74 @@ def test_mx4_product_nan_blocks(b200, m):
     want = ref.mx4_values(ca, sa, d) @ ref.mx4_values(cb, sb, d).T
     np.testing.assert_array_equal(np.isnan(got), bad)
     np.testing.assert_array_equal(got[~bad], want[~bad].astype(np.float32))
+
+
+@pytest.mark.parametrize("m, n, d", [(1, 3000, 768), (3, 260, 4096), (100, 700, 1000), (140, 300, 2048), (1500, 3500, 160)])
+def test_mx4_product_captured_and_on_two_streams(b200, m, n, d):
+    """Every kernel of the product (few rows, split K, 128 and 256 columns, pairs of CTAs): captured once, replayed on
+    other operands in the same memory, while another stream computes a product of its own."""
+    rng = np.random.default_rng(m)
+    mk = lambda r: [torch.from_numpy(t).cuda() for t in ref.mx4_pack(*ref.random_mx4(rng, r, d, 1))]  # noqa: E731
+    a, bb, a2 = mk(m), mk(n), mk(m)
+    out, other = torch.zeros(m, n, device="cuda"), torch.zeros(n, m, device="cuda")
+    call = lambda x, y, r, c, o, s: b200.mx4_product_device(r, c, d, x[0].data_ptr(), x[1].data_ptr(), y[0].data_ptr(),  # noqa: E731
+                                                            y[1].data_ptr(), b200.F32, o.data_ptr(), stream_ptr=s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(a, bb, m, n, out, _stream())
+    vals = lambda t, r: ref.mx4_values(*ref.mx4_unpack(t[0].cpu().numpy(), t[1].cpu().numpy(), r, -(-d // 32)), d)  # noqa: E731
+    vb = vals(bb, n)
+    side = torch.cuda.Stream()
+    for new in (a, a2):
+        if new is not a:
+            for t, u in zip(a, new):
+                t.copy_(u)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            g.replay()
+            call(bb, a, n, m, other, side.cuda_stream)
+        torch.cuda.synchronize()
+        want = vals(a, m) @ vb.T
+        tol = 2 * ref.EPS[0] * d * 36 * 4   # (d > 1800: sums may round)
+        assert float((out.double().cpu() - torch.from_numpy(want)).abs().max()) <= (0 if d <= 1800 else tol)
+        assert torch.equal(other.t(), out) or d > 1800
+
+
+def test_offsets_beyond_32_bits(b200):
+    """More than 2^32 elements of input and of output."""
+    n, d = 70_000_000, 64
+    x = torch.zeros(n, d, dtype=torch.bfloat16, device="cuda")
+    ends = torch.from_numpy(np.random.default_rng(1).standard_normal((300, d))).to("cuda", torch.bfloat16)
+    x[:300], x[-300:] = ends, ends
+    x[33_554_400:33_554_700] = ends            # around element 2^31
+    codes = torch.empty(n, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(b200.mx4_scale_bytes(n, d), dtype=torch.uint8, device="cuda")
+    b200.mx4_quantize_device(n, d, b200.BF16, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), stream_ptr=_stream())
+    rc, rs = ref.mx4_encode(ends.double().cpu().numpy())
+    packed = torch.from_numpy(ref.mx4_pack(rc, rs)[0]).cuda()
+    for lo in (0, 33_554_400, n - 300):
+        assert torch.equal(codes[lo:lo + 300], packed)
+    out = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    b200.mx4_dequantize_device(n, d, codes.data_ptr(), scales.data_ptr(), b200.BF16, out.data_ptr(), stream_ptr=_stream())
+    want = torch.from_numpy(ref.mx4_values(rc, rs, d)).to("cuda", torch.bfloat16)
+    for lo in (0, 33_554_400, n - 300):
+        assert torch.equal(out[lo:lo + 300], want)
+    w = torch.ones(d, dtype=torch.bfloat16, device="cuda")
+    q = torch.empty(n, d, dtype=torch.int8, device="cuda")
+    sc = torch.empty(n, device="cuda")
+    b200.rms_norm_i8_device(n, d, b200.BF16, x.data_ptr(), w.data_ptr(), 1e-6, q.data_ptr(), scales_ptr=sc.data_ptr(), stream_ptr=_stream())
+    check_rms(ends, w, 1e-6, q[-300:], sc[-300:], None)
+    b200.i8_dequantize_device(n, d, q.data_ptr(), b200.BF16, out.data_ptr(), scales_ptr=sc.data_ptr(), stream_ptr=_stream())
+    assert torch.equal(out[-300:], (q[-300:].float() * sc[-300:, None]).bfloat16())
+    del out, q, x
+    # scores: 70 million rows against 70 of them
+    m = 70
+    res = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    b200.mx4_product_device(m, n, d, codes.data_ptr(), scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), b200.BF16,
+                            res.data_ptr(), stream_ptr=_stream())
+    v = want.double()
+    assert torch.equal(res[:, -300:], (v[:m] @ v.t()).bfloat16())
+    assert torch.equal(res[:, :300], (v[:m] @ v.t()).bfloat16())
 
 
 # ---- the operators as they are used ----
