@@ -617,18 +617,16 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
                     const int steps = min(4, (p.nb - 8 * kc + 1) / 2);   // 64 elements each
                     if (leader) {
 #pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                            if (2 * g < steps)
+                        for (int ks = 0; ks < 4; ++ks) {
+                            if (ks >= steps) continue;
+                            const uint32_t col = slot + (ks >> 1) * 12;
+                            if ((ks & 1) == 0)
 #pragma unroll
                                 for (int h = 0; h < 3; ++h)
-                                    ptx::tmem_cp_scales_pair(slot + g * 12 + 4 * h, sf_hi | static_cast<uint64_t>(sf_lo + 64 * h + 32 * g));
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) {
-                            const uint32_t col = slot + (ks >> 1) * 12;
-                            if (ks < steps)
-                                ptx::umma_mxf4_pair(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
-                                                    desc_hi | static_cast<uint64_t>(st + (kPairHalf >> 4) + ks * 2),
-                                                    (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
+                                    ptx::tmem_cp_scales_pair(col + 4 * h, sf_hi | static_cast<uint64_t>(sf_lo + 64 * h + 16 * ks));
+                            ptx::umma_mxf4_pair(tacc, desc_hi | static_cast<uint64_t>(st + ks * 2),
+                                                desc_hi | static_cast<uint64_t>(st + (kPairHalf >> 4) + ks * 2),
+                                                (ks & 1) ? kIdesc2 : kIdesc0, col, col + 4, (kc | ks) ? 1u : 0u);
                         }
                         ptx::umma_commit_pair(&bar_empty[s]);
                         if (kc + 1 == chunks) ptx::umma_commit_pair(&bar_acc_full[t & 1u]);
