@@ -319,7 +319,12 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
                     for (int e = 0; e < 8; ++e) v[j][e] = fminf(fmaxf(v[j][e], -cut), cut);
             }
         } else {
-            if (t == 0 && real) a.scales[row] = top / root / 127.f;
+            if (t == 0 && real) {
+                // the scale to the last bit of fp32, since the values that users take back carry its error: 1 / root by
+                // one step of Newton's method in 64 bits
+                const double ms = ssq / a.d + static_cast<double>(a.eps), r0 = rsqrtf(static_cast<float>(ms));
+                a.scales[row] = static_cast<float>(most * (r0 * (1.5 - 0.5 * ms * r0 * r0)) * (1. / 127.));
+            }
             if (top > 0.f) c = 127.f / top;
         }
         if (!real) continue;
@@ -821,9 +826,9 @@ cudaError_t rms_rows(const RmsNormArgs& a, cudaStream_t st) {
         if (a.d > 2048 && a.d <= 4096) return rms_launch<T, VEC, RES, 128, 4, 6>(a, st);
     }
     if constexpr (sizeof(T) == 2) {
-        if (a.d <= 128) return rms_launch<T, VEC, RES, 8, 2, 6>(a, st);
-        if (a.d <= 256) return rms_launch<T, VEC, RES, 16, 2, 6>(a, st);
-        if (a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 6>(a, st);
+        if (a.d <= 128) return rms_launch<T, VEC, RES, 8, 2, RES ? 4 : 5>(a, st);
+        if (a.d <= 256) return rms_launch<T, VEC, RES, 16, 2, 4>(a, st);
+        if (a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 5>(a, st);
         if (a.d <= 768) return rms_launch<T, VEC, RES, 32, 3, 4>(a, st);
         if (a.d <= 1024) return rms_launch<T, VEC, RES, 64, 2, 12>(a, st);
         if (a.d <= 2048) return rms_launch<T, VEC, RES, 128, 2, 6>(a, st);
