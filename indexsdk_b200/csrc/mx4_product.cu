@@ -110,6 +110,8 @@ __device__ __forceinline__ void finish(const ProductArgs& p, bool owns_tmem, uin
         ptx::tmem_dealloc(tmem_base, 512);
     }
     if (p.split > 1) {
+        if (abort_flag)   // (a copy that landed late may have overwritten the part)
+            for (int e = threadIdx.x; e < TN * kLanes; e += THREADS) reinterpret_cast<uint32_t*>(smem)[e] = 0x7fffffffu;
         ptx::cluster_sync();
         // this CTA's share of the tile's columns: the parts in order of K
         const int c0 = TN * part / p.split, c1 = TN * (part + 1) / p.split;

@@ -698,50 +698,43 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(uint32_t total, Div
         }
         return;
     }
-    for (; i < total; i += 2 * step) {   // two pieces at a time: their loads are on the way together
-        uint32_t w0[2], w1[2], w2[2], k[2];
-        uint32_t s0[2], s1[2], s2[2];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const uint32_t at = i + p * step;
-            if (at + 8 > total) continue;
-            const uint32_t r = by.quotient(at);
-            const int64_t row = row0 + r;
-            k[p] = at - r * by.d;
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + row * pitch) + (k[p] >> 3);
-            const bool ends = k[p] + 8 > by.d;   // (d >= 8)
-            const uint32_t b = k[p] >> 5, b2 = min((k[p] + 7) >> 5, static_cast<uint32_t>(nb - 1));
-            w0[p] = __ldg(w);
-            w1[p] = (k[p] & 7u) && (k[p] >> 3) + 1 < 4u * nb ? __ldg(w + 1) : 0u;
-            w2[p] = ends ? __ldg(reinterpret_cast<const uint32_t*>(codes + (row + 1) * pitch)) : 0u;
-            s0[p] = __ldg(scales + mx4_scale_word(row, b >> 2, ng) + (b & 3u));
-            s1[p] = b2 == b ? s0[p] : __ldg(scales + mx4_scale_word(row, b2 >> 2, ng) + (b2 & 3u));
-            s2[p] = ends ? __ldg(scales + mx4_scale_word(row + 1, 0, ng)) : 0u;
+    const int64_t granule = static_cast<int64_t>(ng) * 512;
+    for (; i < total; i += step) {
+        const uint32_t r = by.quotient(i), k = i - r * by.d, rest = by.d - k;   // rest: elements up to the row's end
+        const int64_t row = row0 + r;
+        if (i + 8 > total) {   // the array's last elements
+            for (uint32_t e = i; e < total; ++e) {
+                const uint32_t re = by.quotient(e);
+                out[e] = from_f<T>(mx4_value(codes + (row0 + re) * pitch, scales, row0 + re, e - re * by.d, ng));
+            }
+            continue;
         }
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + row * pitch) + (k >> 3);
+        const uint8_t* srow = scales + (row >> 7) * granule + (row & 31) * 16 + (row >> 5 & 3) * 4;
+        const uint32_t last = static_cast<uint32_t>(nb - 1), b = k >> 5, b2 = min((k + 7) >> 5, last);
+        const uint32_t w0 = __ldg(w), w1 = (k & 7u) && (k >> 3) < 4 * last + 3 ? __ldg(w + 1) : 0u;
+        const float f0 = e8m0_value(__ldg(srow + (b >> 2) * 512 + (b & 3u)));
+        const float f1 = e8m0_value(__ldg(srow + (b2 >> 2) * 512 + (b2 & 3u)));
+        uint32_t c = __funnelshift_r(w0, w1, 4 * (k & 7u));
+        const uint32_t first = 32u - (k & 31u);   // elements of the first block
+        float f[8];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const uint32_t at = i + p * step;
-            if (at + 8 <= total) {
-                const uint32_t rest = by.d - k[p];   // elements up to the row's end
-                uint32_t c = __funnelshift_r(w0[p], w1[p], 4 * (k[p] & 7u));
-                if (rest < 8) c = (c & ((1u << (4 * rest)) - 1u)) | w2[p] << (4 * rest);
-                const uint32_t first = 32u - (k[p] & 31u);   // elements of the first block
-                const float f0 = e8m0_value(s0[p]), f1 = e8m0_value(s1[p]), f2 = e8m0_value(s2[p]);
-                float f[8];
+        for (uint32_t e = 0; e < 8; e += 2) {
+            const float2 v = e2m1_values(c >> (4 * e));
+            f[e] = v.x * (e < first ? f0 : f1);
+            f[e + 1] = v.y * (e + 1 < first ? f0 : f1);
+        }
+        if (rest < 8) {   // the row ends here (d >= 8): the others come from the next row's first block
+            c = __ldg(reinterpret_cast<const uint32_t*>(codes + (row + 1) * pitch)) << (4 * rest);
+            const float f2 = e8m0_value(__ldg(scales + mx4_scale_word(row + 1, 0, ng)));
 #pragma unroll
-                for (uint32_t e = 0; e < 8; e += 2) {
-                    const float2 v = e2m1_values(c >> (4 * e) & 255u);
-                    f[e] = v.x * (e >= rest ? f2 : (e < first ? f0 : f1));
-                    f[e + 1] = v.y * (e + 1 >= rest ? f2 : (e + 1 < first ? f0 : f1));
-                }
-                store8<T>(out + at, f);
-            } else {
-                for (uint32_t e = at; e < total; ++e) {
-                    const uint32_t r = by.quotient(e);
-                    out[e] = from_f<T>(mx4_value(codes + (row0 + r) * pitch, scales, row0 + r, e - r * by.d, ng));
-                }
+            for (uint32_t e = 0; e < 8; e += 2) {
+                const float2 v = e2m1_values(c >> (4 * e));
+                if (e >= rest) f[e] = v.x * f2;
+                if (e + 1 >= rest) f[e + 1] = v.y * f2;
             }
         }
+        store8<T>(out + i, f);
     }
 }
 
