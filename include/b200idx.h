@@ -199,6 +199,11 @@ int b200idx_mx4_product_device(int64_t m, int64_t n, int d, const uint8_t* a_cod
                                const uint8_t* b_codes, const uint8_t* b_scales, int dtype, void* out, int64_t ldo,
                                void* stream);
 
+/* All inner products of n queries with the rows of an MX4 index (whatever its metric): out[i][p] for the row at
+ * position p, in add order (b200idx_get_ids gives the labels).  x: float, rounded like the rows; x and out are
+ * pointers on the index's device, ready when the call is made; returns when the scores are there. */
+int b200idx_scores_device(b200idx_t* h, int64_t n, const float* x, int dtype, void* out, int64_t ldo);
+
 /* ---- reset / remove_ids / bookkeeping: FR/ascend/AscendIndex.h:77,91;
  *      getBaseSize / getBase / getIdxMap FR/ascend/AscendIndexFlat.h:69-75,
  *      FR/ascend/AscendIndexInt8Flat.h:78-84. ---- */

@@ -78,6 +78,7 @@ def load() -> C.CDLL:
         "b200idx_rms_norm_i8_device": (i32, [i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, vp, i64, vp, vp]),
         "b200idx_add_states_device": (i32, [vp, i64, i32, vp, vp, vp, C.c_float, vp, vp]),
         "b200idx_search_states_device": (i32, [vp, i64, i32, vp, vp, vp, C.c_float, vp, i32, vp, vp]),
+        "b200idx_scores_device": (i32, [vp, i64, vp, i32, vp, i64]),
         "b200idx_i8_dequantize_device": (i32, [i64, i32, vp, i64, vp, vp, i32, vp, i64, vp]),
         "b200idx_mx4_row_bytes": (i64, [i32]),
         "b200idx_mx4_scale_bytes": (i64, [i64, i32]),
@@ -133,7 +134,7 @@ EXPORTED_SYMBOLS = [
     "b200idx_ivfpq_search_preassigned_device", "b200idx_ivfpq_get_nprobe", "b200idx_ivfpq_list_length",
     "b200idx_ivfpq_get_list", "b200idx_stats", "b200idx_set_timing", "b200idx_stream", "b200idx_last_error",
     "b200idx_status_of_message",
-    "b200idx_rms_norm_i8_device", "b200idx_add_states_device", "b200idx_search_states_device", "b200idx_i8_dequantize_device", "b200idx_mx4_row_bytes", "b200idx_mx4_scale_bytes",
+    "b200idx_scores_device", "b200idx_rms_norm_i8_device", "b200idx_add_states_device", "b200idx_search_states_device", "b200idx_i8_dequantize_device", "b200idx_mx4_row_bytes", "b200idx_mx4_scale_bytes",
     "b200idx_mx4_quantize_device", "b200idx_mx4_dequantize_device", "b200idx_mx4_product_device",
     "b200idx_version",
 ]
@@ -284,6 +285,10 @@ class IndexFlat(_Index):
         I = np.empty((n, k), np.int64)
         _check(self._lib.b200idx_search_f16(self._h, n, _ptr(x), k, _ptr(D), _ptr(I)), self._h)
         return D, I
+
+    def scores_device(self, x_ptr: int, n: int, dtype: int, out_ptr: int, ldo: int = 0):
+        """All inner products of n float queries with the rows of an MX4 index, [n][ntotal] in dtype."""
+        _check(self._lib.b200idx_scores_device(self._h, n, x_ptr, dtype, out_ptr, ldo), self._h)
 
     def get_base(self, offset: int = 0, n: int | None = None):
         n = self.ntotal - offset if n is None else n

@@ -202,6 +202,17 @@ void FlatIndex::search_states(int64_t nq, int states_dtype, RmsNormArgs a, int k
     search_device(nq, a.q, false, k, D, I, k);
 }
 
+void FlatIndex::scores_device(int64_t nq, const float* xq, int out_dtype, void* out, int64_t ldo) {
+    if (n_ == 0) return;
+    DeviceGuard g(device_);
+    uint8_t* qop = static_cast<uint8_t*>(w_qop_.ensure(static_cast<size_t>(nq) * op_row_bytes()));
+    uint8_t* qsc = static_cast<uint8_t*>(w_qsc_.ensure(static_cast<size_t>(mx4_scale_bytes(nq, d_))));
+    B200_CUDA_CHECK(launch_mx4_quantize(kF32, nq, d_, xq, d_, 0, qop, qsc, nullptr, stream_));
+    launch_mx4_product(out_dtype, Mx4ProductArgs{nq, n_, d_, qop, qsc, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), out, ldo}, num_sms_, stream_);
+    stats_.kernel_launches += 2;
+    B200_CUDA_CHECK(cudaStreamSynchronize(stream_));
+}
+
 size_t FlatIndex::mx4_file_row() const { return static_cast<size_t>(mx4_pitch(d_)) + mx4_blocks(d_); }
 
 void FlatIndex::get_mx4_rows(int64_t offset, int64_t n, uint8_t* out) const {

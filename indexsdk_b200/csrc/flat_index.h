@@ -117,6 +117,8 @@ public:
     // a.scales are filled in here).
     void add_states(int64_t n, int states_dtype, RmsNormArgs a, const int64_t* ids);
     void search_states(int64_t nq, int states_dtype, RmsNormArgs a, int k, float* D, int64_t* I);
+    // kMX4: all inner products of nq float queries with the rows, out[nq][ldo] in out_dtype, positions along a row.
+    void scores_device(int64_t nq, const float* xq, int out_dtype, void* out, int64_t ldo);
     void reset();
     int64_t remove_ids(int64_t n, const int64_t* ids);
     // Copies rows [offset, offset + n) to a host buffer: float for kF32, fp16 bits for kF16,

@@ -164,6 +164,20 @@ int b200idx_i8_dequantize_device(int64_t n, int d, const int8_t* q, int64_t ldq,
     });
 }
 
+int b200idx_scores_device(b200idx_t* h, int64_t n, const float* x, int dtype, void* out, int64_t ldo) {
+    if (!h) return B200IDX_ERR_INVALID_PARAM;
+    return b200_capi::guarded(h, [&] {
+        FlatIndex* ix = b200_capi::flat_of(h);
+        if (!ix || ix->dtype() != kMX4) throw std::invalid_argument("scores apply to MX4 indexes");
+        check_rows(n, "n");
+        const size_t eb = elem_bytes(dtype);
+        if (ldo != 0 && ldo < ix->ntotal()) throw std::invalid_argument("ldo must be 0 or >= ntotal");
+        if (device_of({{"x", x, 4}, {"out", out, eb}}) != ix->device())
+            throw std::invalid_argument("x and out must lie on the index's device");
+        ix->scores_device(n, x, dtype, out, ldo ? ldo : ix->ntotal());
+    });
+}
+
 int64_t b200idx_mx4_row_bytes(int d) { return d <= 0 || d > kMaxRowElems ? -1 : mx4_pitch(d); }
 int64_t b200idx_mx4_scale_bytes(int64_t n, int d) {
     return n <= 0 || n >= kMaxRows || d <= 0 || d > kMaxRowElems ? -1 : mx4_scale_bytes(n, d);

@@ -165,6 +165,21 @@ def test_several_indexes_together(b200):
     check(b200.search_multi(ixs, q, 25), expected(b200, b200.METRIC_L2, rounded(np.concatenate(parts)), rounded(q), 25))
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n, nq, d, ldo", [(1, 1, 16, 0), (3001, 5, 96, 3008), (700, 200, 1024, 0), (20000, 300, 64, 0)])
+def test_scores(b200, n, nq, d, ldo, dtype):
+    x, q = data(30, n, nq, d)
+    ix = b200.IndexFlat(d, b200.METRIC_L2, b200.MX4)
+    ix.add(x)
+    qd = torch.from_numpy(q).cuda()
+    out = torch.full((nq, ldo or n), -1.0, dtype=ref.TORCH[dtype], device="cuda")
+    torch.cuda.synchronize()
+    ix.scores_device(qd.data_ptr(), nq, dtype, out.data_ptr(), ldo)
+    want = torch.from_numpy(rounded(q) @ rounded(x).T).to(ref.TORCH[dtype])
+    assert torch.equal(out[:, :n].cpu(), want) and bool((out[:, n:] == -1.0).all())
+    check(ix.search(q, 4), expected(b200, b200.METRIC_L2, rounded(x), rounded(q), 4))   # (the scratch is shared)
+
+
 def test_refusals(b200):
     ix = b200.IndexFlat(64, b200.METRIC_L2, b200.MX4)
     x = np.zeros((2, 64), np.float32)
@@ -176,6 +191,13 @@ def test_refusals(b200):
             call()
         assert e.value.code == 2001
     d = torch.zeros(2, 64, device="cuda")
+    for bad in (dict(n=0), dict(x_ptr=0), dict(dtype=b200.MX4), dict(out_ptr=0), dict(ldo=1)):
+        with pytest.raises(b200.B200IdxError) as e:
+            ix.scores_device(**dict(dict(x_ptr=d.data_ptr(), n=2, dtype=b200.F32, out_ptr=d.data_ptr()), **bad))
+        assert e.value.code == 2001
+    with pytest.raises(b200.B200IdxError) as e:
+        b200.IndexFlat(64).scores_device(d.data_ptr(), 2, b200.F32, d.data_ptr())
+    assert e.value.code == 2001 and "MX4" in e.value.msg
     D, I = torch.empty(2, 1, device="cuda"), torch.empty(2, 1, dtype=torch.int64, device="cuda")
     with pytest.raises(b200.B200IdxError) as e:
         ix.search_device_noalloc(d.data_ptr(), 2, 1, D.data_ptr(), I.data_ptr())
