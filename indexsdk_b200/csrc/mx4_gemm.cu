@@ -358,6 +358,10 @@ cudaError_t launch_mx4_dist(const GemmLaunch& L, const GemmArgs& a, const uint8_
     m.nb = mx4_blocks(a.d);
     m.ng = mx4_groups(a.d);
     const bool l2 = a.metric == kMetricL2;
+    if (L.mode == kModeAppend && !a.direct && a.tile_first >= 0 && a.tile_step <= 1) {
+        const cudaError_t e = launch_mx4_few_search(a, a_scales, b_scales, L.num_sms, stream);
+        if (e != cudaErrorNotSupported) return e;
+    }
     if (L.mode == kModeAppend)
         return l2 ? launch_one<kModeAppend, 32, true>(m, mapA, mapB, L.num_sms, stream)
                   : launch_one<kModeAppend, 32, false>(m, mapA, mapB, L.num_sms, stream);

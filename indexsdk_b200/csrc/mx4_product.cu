@@ -62,7 +62,13 @@ struct ProductArgs {
     int64_t ldo;
     int a_tiles, b_tiles;    // tiles of TN rows of a, of 128 rows of b
     int split;               // CTAs of a cluster that share a tile's K (1: none)
+    int b_first;             // mx4_few_kernel: first tile of b
+    GemmArgs g;              // mx4_few_kernel as a pass of a search: thresholds and candidate lists
 };
+
+// What mx4_few_kernel does with its accumulators: scores to memory, or a search's keys at or below the row's threshold
+// to its candidate list (inner product, L2).
+enum FewEnd : int { kEndStore, kEndSearchIP, kEndSearchL2 };
 
 __device__ __forceinline__ void next_tile(const ProductArgs& p, int& bt, int& at) {
     if (++at == p.a_tiles) {
@@ -307,7 +313,45 @@ struct Few {
     static constexpr int resident_bytes(int chunks) { return chunks * (TN * kChunk + 1024); }
 };
 
-template <int TN, typename T>
+// A warp's 32 rows of b against COLS queries, accumulators at tacc, values in r: candidates into the queries' lists.
+// Rows are lanes here, so a row's norm is one register and a hit's slots are taken for all lanes that have the same
+// query in one atomic; 32 queries' atomics are on their way together.  A query's threshold is read from shared memory.
+template <bool L2, int COLS>
+__device__ __forceinline__ void take_candidates(const uint32_t (&r)[COLS], const GemmArgs& a, const float* tau, int first, uint32_t tacc,
+                                                int64_t j, float norm) {
+    uint32_t pass[2] = {0u, 0u};
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+        const float v = __uint_as_float(r[c]);
+        if ((L2 ? fmaf(-2.f, v, norm) : -v) <= tau[c]) pass[c >> 5] |= 1u << (c & 31);   // (NaN is not)
+    }
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < (COLS + 31) / 32; ++h) {
+        uint32_t mine = j < a.N ? pass[h] : 0u;
+        uint32_t who = 0u;   // lanes with a candidate of query 32 h + lane
+        for (uint32_t any = __reduce_or_sync(0xFFFFFFFFu, mine); any; any &= any - 1) {
+            const int c = __ffs(any) - 1;
+            if (a.qmask && (mine >> c & 1u) &&
+                !(__ldg(a.qmask + static_cast<int64_t>(first + 32 * h + c) * a.qmask_stride + (j >> 5)) >> (j & 31) & 1u))
+                mine &= ~(1u << c);
+            const uint32_t w = __ballot_sync(0xFFFFFFFFu, mine >> c & 1u);
+            if (lane == c) who = w;
+        }
+        uint32_t slots = 0;
+        if (who) slots = atomicAdd(a.counts + first + 32 * h + lane, static_cast<uint32_t>(__popc(who)));
+        for (uint32_t any = __ballot_sync(0xFFFFFFFFu, who != 0u); any; any &= any - 1) {
+            const int c = __ffs(any) - 1;
+            const float v = __uint_as_float(ptx::tmem_ld_32x1(tacc + 32 * h + c));
+            const uint32_t slot = __shfl_sync(0xFFFFFFFFu, slots, c) + __popc(__shfl_sync(0xFFFFFFFFu, who, c) & ((1u << lane) - 1u));
+            const float key = L2 ? fmaf(-2.f, v, norm) : -v;
+            if ((mine >> c & 1u) && slot < a.cap)
+                a.cand[static_cast<int64_t>(first + 32 * h + c) * a.cap + slot] = pack_cand(float_to_ord(key), static_cast<uint32_t>(j));
+        }
+    }
+}
+
+template <int TN, typename T, int END = kEndStore>
 __global__ void __launch_bounds__(kFewThreads, 1)
 mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
                const __grid_constant__ ProductArgs p, const int half_stages) {
@@ -315,14 +359,15 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[kFewMaxStages], bar_empty[kFewMaxStages], bar_acc_full[K::kAcc], bar_acc_free[K::kAcc], bar_a, bar_a_scales;
     __shared__ uint32_t tmem_base_slot;
+    __shared__ __align__(16) float tau[END == kEndStore ? 1 : TN];
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int chunks = (p.ng + 1) / 2;
     const int workers = gridDim.x / p.split, worker = blockIdx.x / p.split;
-    const int lo = static_cast<int>(static_cast<int64_t>(p.b_tiles) * worker / workers);
-    const int hi = static_cast<int>(static_cast<int64_t>(p.b_tiles) * (worker + 1) / workers);
+    const int lo = p.b_first + static_cast<int>(static_cast<int64_t>(p.b_tiles) * worker / workers);
+    const int hi = p.b_first + static_cast<int>(static_cast<int64_t>(p.b_tiles) * (worker + 1) / workers);
     const int part = p.split > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
     const int kc0 = chunks * part / p.split, kc1 = chunks * (part + 1) / p.split, nkc = kc1 - kc0;
     uint8_t* a_codes = smem;                              // [nkc][TN][128 B]
@@ -344,6 +389,8 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
         ptx::prefetch_tensormap(&map_a);
         ptx::prefetch_tensormap(&map_b);
     }
+    if (END != kEndStore && threadIdx.x < TN)   // (columns behind the last query let nothing pass)
+        tau[threadIdx.x] = threadIdx.x < p.m ? ord_to_float(__ldg(p.g.tau + threadIdx.x)) : __int_as_float(0x7fffffff);
     if (warp == 2) {
         ptx::tmem_alloc(&tmem_base_slot, 512);
         ptx::tmem_relinquish();
@@ -436,7 +483,9 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
         for (int bt = lo + ab; bt < hi; bt += K::kAcc, ++turn) {
             const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
             uint32_t r[K::kCols];
+            const float norm = END == kEndSearchL2 ? __ldg(static_cast<const float*>(p.g.bnorm) + j) : 0.f;
             if (ok) ok = ptx::mbar_wait_warp(&bar_acc_full[ab], turn & 1u, &abort_flag);
+            if (END != kEndStore && !ok) break;   // (the host sees the error word)
             if (ok) {
                 ptx::tc_fence_after();
                 const uint32_t tacc = tmem_base + ab * TN + first + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -449,9 +498,12 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
                     ptx::tmem_ld_32x16(tacc, r);
                     ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[16]>(r));
                 }
+                if constexpr (END != kEndStore)
+                    take_candidates<END == kEndSearchL2>(r, p.g, tau + first, first, tacc, j, norm);
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&bar_acc_free[ab]);
+                if (END != kEndStore) continue;
             } else {
                 // (as above: no numbers)
 #pragma unroll
@@ -467,6 +519,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     }
 
     finish<kFewThreads, TN, T>(p, warp == 2, tmem_base, abort_flag, smem, lo, 0, part);
+    if (END != kEndStore && threadIdx.x == 0 && abort_flag) atomicOr(p.g.err, kDevErrPipelineTimeout);
 }
 
 template <int TN, typename T>
@@ -744,6 +797,56 @@ void launch_mx4_product(int dtype, const Mx4ProductArgs& q, int num_sms, cudaStr
     if (dtype == kF32) product<float>(q, num_sms, st);
     else if (dtype == kF16) product<__half>(q, num_sms, st);
     else product<__nv_bfloat16>(q, num_sms, st);
+}
+
+namespace {
+template <int TN, int END>
+cudaError_t few_search(const ProductArgs& p, const CUtensorMap& map_b, const CUtensorMap& map_a, int num_sms, int half, cudaStream_t st) {
+    auto kern = mx4_few_kernel<TN, float, END>;
+    cudaError_t e = allow_max_smem(kern);
+    if (e != cudaSuccess) return e;
+    const int chunks = (p.ng + 1) / 2;
+    const int grid = std::min(p.b_tiles, num_sms);
+    kern<<<grid, kFewThreads, 1024 + Few<TN>::resident_bytes(chunks) + 2 * half * kFewStage, st>>>(map_b, map_a, p, half);
+    return cudaGetLastError();
+}
+template <int TN>
+cudaError_t few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales, int num_sms, cudaStream_t st) {
+    ProductArgs p{};
+    p.a_scales = a_scales;
+    p.b_scales = b_scales;
+    p.nb = mx4_blocks(a.d);
+    p.ng = mx4_groups(a.d);
+    p.m = a.nq;
+    p.n = a.N;
+    p.split = 1;
+    p.a_tiles = 1;
+    p.b_first = a.tile_first * (kTileB / kLanes);
+    p.b_tiles = std::min(a.n_tiles_sel * (kTileB / kLanes), div_up(a.N, kLanes) - p.b_first);
+    p.g = a;
+    if (p.b_tiles <= 0) return cudaSuccess;
+    const int chunks = (p.ng + 1) / 2;
+    const int half = std::min(kFewMaxStages, (kSmemMost - 1024 - Few<TN>::resident_bytes(chunks)) / kFewStage) / 2;
+    if (chunks > Few<TN>::kMaxChunks || half < 3) return cudaErrorNotSupported;
+    CUtensorMap map_a, map_b;
+    if (encode_mx4_map(&map_a, static_cast<const uint8_t*>(a.A), a.nq, a.d, TN) != 0 ||
+        encode_mx4_map(&map_b, static_cast<const uint8_t*>(a.B), a.N, a.d, kLanes) != 0)
+        return cudaErrorInvalidValue;
+    return a.metric == kMetricL2 ? few_search<TN, kEndSearchL2>(p, map_b, map_a, num_sms, half, st)
+                                 : few_search<TN, kEndSearchIP>(p, map_b, map_a, num_sms, half, st);
+}
+}  // namespace
+
+// Against 1 M rows, the other kernel's pass and this one's: 1 query x 128 L2 74 and 35 us (its tile has 128 lanes for
+// queries, and every lane tests); 16 x 256 L2 84 and 46; 64 x 128 inner product 73 and 58; 64 x 768 98 and 93, where the
+// rows' bytes take 54.
+cudaError_t launch_mx4_few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales, int num_sms, cudaStream_t st) {
+    if (a.nq <= 16) return few_search<16>(a, a_scales, b_scales, num_sms, st);
+    if (a.nq <= 32) return few_search<32>(a, a_scales, b_scales, num_sms, st);
+    if (a.nq <= 64) return few_search<64>(a, a_scales, b_scales, num_sms, st);
+    // (the other kernel wins by 10 us there without norms, this one by as much with them: 100 queries, 1 M x 768)
+    if (a.nq <= 128 && a.metric == kMetricL2) return few_search<128>(a, a_scales, b_scales, num_sms, st);
+    return cudaErrorNotSupported;
 }
 
 int encode_mx4_map(CUtensorMap* out, const uint8_t* codes, int64_t rows, int d, int box_rows) {

@@ -335,6 +335,11 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ uint32_t tmem_ld_32x1(uint32_t taddr) {   // one column, waited for
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+    return r;
+}
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t* r) {   // 16 columns
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "

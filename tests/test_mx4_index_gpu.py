@@ -105,6 +105,27 @@ def test_masks(b200, metric):
 
 
 @pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("n, nq, d, k", [(140001, 16, 48, 10), (140001, 17, 32, 200), (140001, 64, 80, 3), (133000, 128, 64, 20),
+                                         (30011, 2, 2064, 10), (30000, 40, 2064, 10)])
+def test_few_queries_over_many_rows(b200, n, nq, d, k, metric):
+    """Thresholds and two stretches of the base; rows that are no numbers; a filter; the same index twice in a row."""
+    x, q = data(n + nq, n, nq, d)
+    x[5, 0], x[n - 1, d - 1] = np.nan, np.inf
+    q[nq - 1] = 0.0
+    ix = b200.IndexFlat(d, metric, b200.MX4)
+    ix.add(x)
+    vb, vq = rounded(x), rounded(q)
+    want = expected(b200, metric, vb, vq, k)
+    check(ix.search(q, k), want)
+    check(ix.search(q, k), want)
+    rng = np.random.default_rng(n)
+    keep = rng.random((nq, n)) < 0.6
+    keep[0] = False
+    keep[0, n - 2] = True
+    check(ix.search_with_masks(q, k, np.packbits(keep, axis=1, bitorder="little")), expected(b200, metric, vb, vq, k, keep))
+
+
+@pytest.mark.parametrize("metric", [0, 1])
 def test_rows_that_are_no_numbers(b200, metric):
     x, q = data(4, 300, 5, 96)
     x[7, 3], x[299, 95], x[100] = np.nan, np.inf, -np.inf
