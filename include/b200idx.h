@@ -51,7 +51,8 @@ enum { B200IDX_F32 = 0, B200IDX_F16 = 1 };
 /*   MX4: float rows in, kept as microscaled 4-bit floating point (see below; 17 bytes for 32 elements), fp32
  *        accumulation.  Queries are rounded the same way: distances and scores are those of the rounded
  *        vectors, ties go to the lower position, a row or query with a block that stands for NaN has no
- *        results.  b200idx_get_base gives the values that the rows stand for.  (No reference counterpart.) */
+ *        results.  b200idx_get_base gives the values that the rows stand for.  At most 2^31 - 256 rows.  (No reference
+ *        counterpart.) */
 enum { B200IDX_MX4 = 4 };
 /* Element type of rows in device memory that the operators below read or write, besides the two above. */
 enum { B200IDX_BF16 = 2 };

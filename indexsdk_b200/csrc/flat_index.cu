@@ -107,6 +107,8 @@ void FlatIndex::reserve(int64_t n) {
 
 void FlatIndex::begin_add(int64_t n) {
     if (n_ + n > 0xFFFFFFF0ll) throw std::invalid_argument("a single-device index holds at most 2^32 - 16 vectors");
+    if (dtype_ == kMX4 && n_ + n > 0x7FFFFF00ll)   // (a row's number is a signed 32-bit coordinate of the tensor map)
+        throw std::invalid_argument("a single-device MX4 index holds at most 2^31 - 256 vectors");
     reserve(n_ + n);
 }
 
