@@ -157,7 +157,8 @@ int b200idx_merge_topk_device_strided(int nsrc, int64_t n, int k, int descending
  *   q = round(y / scale) to nearest, ties to even, cut to [-127, 127];  q has row stride ldq
  *   scale: static_scale[0] where that is given, else max|y| / 127 of the row, written to scales[n]
  * (exactly one of scales and static_scale is NULL).  A row of zeros has scale 0 and q 0.  A row with a NaN or
- * an infinity has q 0 and scale NaN; a static scale that is not a positive number gives q 0. */
+ * an infinity has q 0 and scale NaN, and so has every row where a weight is one; a static scale that is not a
+ * positive number gives q 0. */
 int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64_t ldx, const void* residual,
                                int64_t ldr, void* sum, int64_t lds, const void* weight, float eps,
                                const float* static_scale, int8_t* q, int64_t ldq, float* scales, void* stream);

@@ -30,6 +30,17 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Eight elements as they lie in memory: four or eight words.
 template <typename T>
 struct Row8 {
@@ -159,8 +170,9 @@ __device__ __noinline__ int hard_row(const RmsNormArgs& a, int64_t row, int t, b
         const int k = VEC ? (t + NT * (i >> 3)) * 8 + (i & 7) : t + NT * i;
         if (!mine || k >= a.d) continue;
         const double s = row_element<T, RES>(a, row, k);
-        ssq += s * s;
-        top = fmax(top, fabs(s * to_f<T>(static_cast<const T*>(a.weight)[k])));
+        const double p = fabs(s * to_f<T>(static_cast<const T*>(a.weight)[k]));
+        ssq += p < __longlong_as_double(0x7ff0000000000000ll) ? s * s : p;   // (a weight that is no number: nor is the row)
+        top = fmax(top, p);
     }
     reduce_row<NT>(ssq, top, sh, turn);
     if (!mine) return turn;
@@ -272,7 +284,8 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             for (int e = 0; e < 8; ++e) {
                 part = fmaf(f[e], f[e], part);
                 v[j][e] = f[e] * w[e];
-                if (kLow && fabsf(v[j][e]) > top) {
+                // (as whole numbers, which puts a NaN above all)
+                if (kLow && (__float_as_uint(v[j][e]) & 0x7fffffffu) > __float_as_uint(top)) {
                     top = fabsf(v[j][e]);
                     top_s = f[e];
                     top_w = w[e];
@@ -286,9 +299,10 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             }
             if (!kLow) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) top = ptx::max3(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
+                for (int e = 0; e < 8; e += 2) top = max_nan(top, fabsf(v[j][e]), fabsf(v[j][e + 1]));
             }
         }
+        if (top != top) ssq = __longlong_as_double(0x7ff8000000000000ll);   // (a weight; reductions of `top` do not pass a NaN on)
         if (kAhead && row + step < a.n) fetch_row(row + step);
         const float mine = top;
         double most = 0.;   // the largest product
@@ -471,17 +485,6 @@ __device__ __forceinline__ float2 e2m1_values(uint32_t byte) {
 }
 __device__ __forceinline__ float e8m0_value(uint32_t byte) {   // 2^(byte - 127), NaN for 255
     return byte == 0u ? __int_as_float(0x00400000) : __int_as_float(byte == 255u ? 0x7fc00000 : byte << 23);
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
 }
 
 // 32 consecutive bytes of a row that starts off a 16-byte boundary: the aligned words around them, shifted.

@@ -211,6 +211,20 @@ def test_rms_norm_range(b200):
         assert bool((q == 0).all())
 
 
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("n, d, dtype", [(5, 20, 0), (7, 100, 1), (6, 128, 2), (3, 777, 2), (4, 900, 0), (3, 4096, 2), (2, 16384, 1)])
+def test_rms_norm_weights_that_are_no_numbers(b200, n, d, dtype, static, bad):
+    rng = np.random.default_rng(d)
+    x = _rows(rng, n, d, dtype)
+    x[n - 1, d // 2] = 0.0   # 0 * infinity
+    w = torch.ones(d, dtype=ref.TORCH[dtype], device="cuda")
+    w[d // 2] = float(bad)
+    q, scales, _ = rms(b200, x, w, static=torch.full((1,), 0.03, device="cuda") if static else None)
+    assert bool((q == 0).all())
+    assert static or bool(torch.isnan(scales).all())
+
+
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("d, dtype", [(20, 0), (100, 1), (100, 2), (128, 0), (250, 2), (500, 1), (900, 2)])
 def test_rms_norm_range_next_to_others(b200, d, dtype, residual):
