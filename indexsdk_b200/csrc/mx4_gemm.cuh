@@ -27,8 +27,8 @@ void launch_mx4_product(int dtype, const Mx4ProductArgs& a, int num_sms, cudaStr
 cudaError_t launch_mx4_dist(const GemmLaunch& L, const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales,
                             const CUtensorMap* mapA, const CUtensorMap* mapB, cudaStream_t stream);
 
-// The same for up to 64 (L2: 128) queries and thresholds (kModeAppend, not direct, consecutive tiles), with the base rows on the
-// accumulator's lanes; cudaErrorNotSupported where the queries do not fit.  A candidate takes one slot of its list.
+// The same for up to 128 queries and thresholds (kModeAppend, not direct, consecutive tiles), with the base rows on the
+// accumulator's lanes; cudaErrorNotSupported where the queries do not fit.
 cudaError_t launch_mx4_few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales, int num_sms, cudaStream_t stream);
 
 // Tensor map of codes: boxes of box_rows rows x 128 bytes (256 elements), SWIZZLE_128B.  0 on success.

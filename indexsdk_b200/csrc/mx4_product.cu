@@ -313,12 +313,25 @@ struct Few {
     static constexpr int resident_bytes(int chunks) { return chunks * (TN * kChunk + 1024); }
 };
 
-// A warp's 32 rows of b against COLS queries, accumulators at tacc, values in r: candidates into the queries' lists.
+// A CTA's candidates wait in shared memory, kNearAll / TN for each query, and go to the queries' lists at the end
+// (or, when there are more, at once).
+constexpr int kNearAll = 2048;
+template <int TN>
+struct NearList {
+    static constexpr int kSlots = kNearAll / TN;
+    uint32_t taken[TN];      // slots reserved, may pass kSlots
+    uint32_t base[TN];
+    float tau[TN];
+};
+// A warp's 32 rows of b against COLS queries, accumulators at tacc, values in r: candidates into `list`.
 // Rows are lanes here, so a row's norm is one register and a hit's slots are taken for all lanes that have the same
-// query in one atomic; 32 queries' atomics are on their way together.  A query's threshold is read from shared memory.
-template <bool L2, int COLS>
-__device__ __forceinline__ void take_candidates(const uint32_t (&r)[COLS], const GemmArgs& a, const float* tau, int first, uint32_t tacc,
-                                                int64_t j, float norm) {
+// query in one atomic, 32 queries' at a time.  In shared memory, since most tiles of a warp have a candidate and
+// would wait for the global counters (64 queries, 1 M x 128, inner product: the passes 58 us with global ones).
+template <bool L2, int TN, int COLS>
+__device__ __forceinline__ void take_candidates(const uint32_t (&r)[COLS], const GemmArgs& a, NearList<TN>& near, uint64_t* list, int first,
+                                                uint32_t tacc, int64_t j, float norm) {
+    constexpr uint32_t kSlots = NearList<TN>::kSlots;
+    const float* tau = near.tau + first;
     uint32_t pass[2] = {0u, 0u};
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
@@ -338,15 +351,23 @@ __device__ __forceinline__ void take_candidates(const uint32_t (&r)[COLS], const
             const uint32_t w = __ballot_sync(0xFFFFFFFFu, mine >> c & 1u);
             if (lane == c) who = w;
         }
-        uint32_t slots = 0;
-        if (who) slots = atomicAdd(a.counts + first + 32 * h + lane, static_cast<uint32_t>(__popc(who)));
+        uint32_t slots = 0;   // of the list in shared memory; from kSlots on: of the query's own
+        if (who) {
+            const uint32_t more = __popc(who);
+            slots = atomicAdd(&near.taken[first + 32 * h + lane], more);
+            if (slots + more > kSlots) slots = kSlots + atomicAdd(a.counts + first + 32 * h + lane, more);
+        }
         for (uint32_t any = __ballot_sync(0xFFFFFFFFu, who != 0u); any; any &= any - 1) {
             const int c = __ffs(any) - 1;
             const float v = __uint_as_float(ptx::tmem_ld_32x1(tacc + 32 * h + c));
             const uint32_t slot = __shfl_sync(0xFFFFFFFFu, slots, c) + __popc(__shfl_sync(0xFFFFFFFFu, who, c) & ((1u << lane) - 1u));
             const float key = L2 ? fmaf(-2.f, v, norm) : -v;
-            if ((mine >> c & 1u) && slot < a.cap)
-                a.cand[static_cast<int64_t>(first + 32 * h + c) * a.cap + slot] = pack_cand(float_to_ord(key), static_cast<uint32_t>(j));
+            if (mine >> c & 1u) {
+                const uint64_t cand = pack_cand(float_to_ord(key), static_cast<uint32_t>(j));
+                const int q = first + 32 * h + c;
+                if (slot < kSlots) list[q * kSlots + slot] = cand;
+                else if (slot - kSlots < a.cap) a.cand[static_cast<int64_t>(q) * a.cap + slot - kSlots] = cand;
+            }
         }
     }
 }
@@ -359,7 +380,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[kFewMaxStages], bar_empty[kFewMaxStages], bar_acc_full[K::kAcc], bar_acc_free[K::kAcc], bar_a, bar_a_scales;
     __shared__ uint32_t tmem_base_slot;
-    __shared__ __align__(16) float tau[END == kEndStore ? 1 : TN];
+    __shared__ __align__(16) NearList<END == kEndStore ? 1 : TN> near;
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -389,8 +410,14 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
         ptx::prefetch_tensormap(&map_a);
         ptx::prefetch_tensormap(&map_b);
     }
-    if (END != kEndStore && threadIdx.x < TN)   // (columns behind the last query let nothing pass)
-        tau[threadIdx.x] = threadIdx.x < p.m ? ord_to_float(__ldg(p.g.tau + threadIdx.x)) : __int_as_float(0x7fffffff);
+    uint64_t* list = reinterpret_cast<uint64_t*>(ring + 2 * half_stages * kFewStage);   // search only
+    if constexpr (END != kEndStore) {
+        if (threadIdx.x < TN) {   // (columns behind the last query let nothing pass)
+            near.tau[threadIdx.x] = threadIdx.x < p.m ? ord_to_float(__ldg(p.g.tau + threadIdx.x)) : __int_as_float(0x7fffffff);
+            near.taken[threadIdx.x] = 0;
+        }
+        for (int e = threadIdx.x; e < kNearAll; e += kFewThreads) list[e] = kCandInvalid;   // (a reservation past the end leaves some)
+    }
     if (warp == 2) {
         ptx::tmem_alloc(&tmem_base_slot, 512);
         ptx::tmem_relinquish();
@@ -480,10 +507,16 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
         bool ok = true;
         float* parts = reinterpret_cast<float*>(smem);           // split: [TN][128]
         uint32_t turn = 0;
+        // (a tile's norms are on their way while the tile before it is worked on)
+        auto norm_of = [&](int bt) {
+            return END == kEndSearchL2 && bt < hi ? __ldg(static_cast<const float*>(p.g.bnorm) + static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane) : 0.f;
+        };
+        float norm = 0.f, next_norm = norm_of(lo + ab);
         for (int bt = lo + ab; bt < hi; bt += K::kAcc, ++turn) {
             const int64_t j = static_cast<int64_t>(bt) * kLanes + quarter * 32 + lane;
             uint32_t r[K::kCols];
-            const float norm = END == kEndSearchL2 ? __ldg(static_cast<const float*>(p.g.bnorm) + j) : 0.f;
+            norm = next_norm;
+            next_norm = norm_of(bt + K::kAcc);
             if (ok) ok = ptx::mbar_wait_warp(&bar_acc_full[ab], turn & 1u, &abort_flag);
             if (END != kEndStore && !ok) break;   // (the host sees the error word)
             if (ok) {
@@ -499,7 +532,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
                     ptx::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[16]>(r));
                 }
                 if constexpr (END != kEndStore)
-                    take_candidates<END == kEndSearchL2>(r, p.g, tau + first, first, tacc, j, norm);
+                    take_candidates<END == kEndSearchL2, TN>(r, p.g, near, list, first, tacc, j, norm);
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&bar_acc_free[ab]);
@@ -519,7 +552,19 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant_
     }
 
     finish<kFewThreads, TN, T>(p, warp == 2, tmem_base, abort_flag, smem, lo, 0, part);
-    if (END != kEndStore && threadIdx.x == 0 && abort_flag) atomicOr(p.g.err, kDevErrPipelineTimeout);
+    if constexpr (END != kEndStore) {   // (finish has brought all threads together)
+        constexpr int kSlots = NearList<TN>::kSlots;
+        if (threadIdx.x < TN && near.taken[threadIdx.x])
+            near.base[threadIdx.x] = atomicAdd(p.g.counts + threadIdx.x, min(near.taken[threadIdx.x], static_cast<uint32_t>(kSlots)));
+        __syncthreads();
+        for (int e = threadIdx.x; e < kNearAll; e += kFewThreads) {
+            const uint32_t q = e / kSlots, i = e % kSlots;
+            if (i >= near.taken[q]) continue;
+            const uint32_t slot = near.base[q] + i;
+            if (slot < p.g.cap) p.g.cand[static_cast<int64_t>(q) * p.g.cap + slot] = list[e];
+        }
+        if (threadIdx.x == 0 && abort_flag) atomicOr(p.g.err, kDevErrPipelineTimeout);
+    }
 }
 
 template <int TN, typename T>
@@ -807,7 +852,7 @@ cudaError_t few_search(const ProductArgs& p, const CUtensorMap& map_b, const CUt
     if (e != cudaSuccess) return e;
     const int chunks = (p.ng + 1) / 2;
     const int grid = std::min(p.b_tiles, num_sms);
-    kern<<<grid, kFewThreads, 1024 + Few<TN>::resident_bytes(chunks) + 2 * half * kFewStage, st>>>(map_b, map_a, p, half);
+    kern<<<grid, kFewThreads, 1024 + Few<TN>::resident_bytes(chunks) + 2 * half * kFewStage + kNearAll * 8, st>>>(map_b, map_a, p, half);
     return cudaGetLastError();
 }
 template <int TN>
@@ -826,7 +871,7 @@ cudaError_t few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t
     p.g = a;
     if (p.b_tiles <= 0) return cudaSuccess;
     const int chunks = (p.ng + 1) / 2;
-    const int half = std::min(kFewMaxStages, (kSmemMost - 1024 - Few<TN>::resident_bytes(chunks)) / kFewStage) / 2;
+    const int half = std::min(kFewMaxStages, (kSmemMost - 1024 - kNearAll * 8 - Few<TN>::resident_bytes(chunks)) / kFewStage) / 2;
     if (chunks > Few<TN>::kMaxChunks || half < 3) return cudaErrorNotSupported;
     CUtensorMap map_a, map_b;
     if (encode_mx4_map(&map_a, static_cast<const uint8_t*>(a.A), a.nq, a.d, TN) != 0 ||
@@ -837,15 +882,14 @@ cudaError_t few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t
 }
 }  // namespace
 
-// Against 1 M rows, the other kernel's pass and this one's: 1 query x 128 L2 74 and 35 us (its tile has 128 lanes for
-// queries, and every lane tests); 16 x 256 L2 84 and 46; 64 x 128 inner product 73 and 58; 64 x 768 98 and 93, where the
-// rows' bytes take 54.
+// Against 1 M rows, the other kernel's passes and this one's: 1 query x 128 L2 75 and 36 us (its tile has 128 lanes for
+// queries, and every lane tests); 64 x 128 inner product 73 and 48; 128 x 128 k = 100 78 and 73; 100 x 768 101 and 100, where
+// the rows' bytes take 62.
 cudaError_t launch_mx4_few_search(const GemmArgs& a, const uint8_t* a_scales, const uint8_t* b_scales, int num_sms, cudaStream_t st) {
     if (a.nq <= 16) return few_search<16>(a, a_scales, b_scales, num_sms, st);
     if (a.nq <= 32) return few_search<32>(a, a_scales, b_scales, num_sms, st);
     if (a.nq <= 64) return few_search<64>(a, a_scales, b_scales, num_sms, st);
-    // (the other kernel wins by 10 us there without norms, this one by as much with them: 100 queries, 1 M x 768)
-    if (a.nq <= 128 && a.metric == kMetricL2) return few_search<128>(a, a_scales, b_scales, num_sms, st);
+    if (a.nq <= 128) return few_search<128>(a, a_scales, b_scales, num_sms, st);
     return cudaErrorNotSupported;
 }
 
