@@ -303,6 +303,19 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             }
         }
         if (top != top) ssq = __longlong_as_double(0x7ff8000000000000ll);   // (a weight; reductions of `top` do not pass a NaN on)
+        // Products below fp32's least number come out as zeros: that number stands for them, so that a row that has nothing
+        // larger is done in 64 bits.  (Rows of zeros, as in a padded batch, stay here.)
+        if (!std::is_same<T, __half>::value && top == 0.f) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) any |= RES ? x[j].w[i] | r[RES ? j : 0].w[i] : x[j].w[i];
+            if (any & (kLow ? 0x7fffffffu : 0x7fff7fffu)) {
+                top = top_s = __int_as_float(1);
+                top_w = 1.f;
+            }
+        }
         if (kAhead && row + step < a.n) fetch_row(row + step);
         const float mine = top;
         double most = 0.;   // the largest product
@@ -314,7 +327,8 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             reduce_row<NT>(ssq, top, sh, turn);
             most = top;
         }
-        const bool hard = !(ssq <= 3e38) || !(top <= 1e36f) || (top < 1e-20f && top > 0.f);
+        // (a given scale this small divides products that are no fp32 numbers)
+        const bool hard = !(ssq <= 3e38) || !(top <= 1e36f) || (top < 1e-20f && top > 0.f) || (a.static_scale && !(__ldg(a.static_scale) >= 1e-30f));
         if (NT < 32 ? __any_sync(0xFFFFFFFFu, hard) : hard) {
             turn = hard_row<T, VEC, RES, NT, J>(a, row, t, hard && real, sh, turn);
             if (hard) continue;
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
         float c = 0.f;   // q = round(v c); 0: zeros
         if (a.static_scale) {
             const float given = __ldg(a.static_scale);
-            if (given > 0.f && given <= 3.4e38f) c = fminf(1.f / root / given, 3e38f);
+            if (given <= 3.4e38f) c = 1.f / root / given;
             if (mine * c > 127.f) {   // (few values: a scale is made for its rows)
                 const float cut = 127.f / c;
 #pragma unroll

@@ -251,6 +251,51 @@ def test_rms_norm_range_next_to_others(b200, d, dtype, residual):
     check_rms(x[good], w, 1e-6, q[good], scales[good], None if total is None else total[good], None if r is None else r[good])
 
 
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n, d, dtype", [(3, 20, 0), (700, 100, 2), (9, 128, 0), (5, 250, 2), (300, 777, 2), (4, 1024, 0), (3, 4096, 2),
+                                         (2, 9000, 0), (2, 16384, 2)])
+def test_rms_norm_products_below_fp32(b200, n, d, dtype, residual, static):
+    """s w below fp32's least number, y above it (the root is at least 1e-6 with this eps): rows between zeros and others."""
+    rng = np.random.default_rng(d)
+    base = rng.uniform(0.25, 1.0, (n, d)) * rng.choice([-1.0, 1.0], (n, d))
+    kind = np.arange(n) % 3
+    base[kind == 0] *= 1e-23            # products of at most 5e-46: no fp32 number but 0 is as near
+    base[kind == 1] = 0
+    x = torch.from_numpy(base).to("cuda", ref.TORCH[dtype])
+    w = torch.from_numpy(rng.uniform(0.5, 1.0, d) * 5e-23).to("cuda", ref.TORCH[dtype])
+    r = torch.zeros_like(x) if residual else None
+    s = torch.full((1,), 1e-41, device="cuda") if static else None
+    q, scales, total = rms(b200, x, w, eps=1e-12, residual=r, static=s)
+    y = ref.rms_norm(x.double().cpu().numpy(), w.double().cpu().numpy(), 1e-12)
+    tiny = kind == 0
+    assert 0 < np.abs(y[tiny]).max() < 2.0 ** -125 and bool((q[torch.from_numpy(kind == 1).cuda()] == 0).all())
+    if static:
+        step = np.full((n, 1), float(s.double()))
+    else:
+        top = np.abs(y).max(1) / 127
+        # half of fp32's least number where the scale is that small
+        np.testing.assert_allclose(scales.double().cpu().numpy(), top, rtol=(d / 64 + 8) * ref.EPS[0], atol=2.0 ** -150)
+        step = np.where(top > 0, top, 1.0)[:, None]
+    assert np.abs(np.clip(y / step, -127, 127)[tiny]).max() > 5
+    off = np.abs(q.double().cpu().numpy() - np.clip(y / step, -127, 127))
+    assert off.max() <= 0.5 + 127 * (d / 64 + 8) * ref.EPS[0], off.max()
+
+
+@pytest.mark.parametrize("d, dtype", [(40, 0), (300, 2), (2048, 0)])
+def test_rms_norm_given_scale_below_fp32(b200, d, dtype):
+    """A given scale of 1e-41: elements of that size count next to large ones, which are cut."""
+    rng = np.random.default_rng(d)
+    x = rng.standard_normal((6, d))
+    x[:, 1::2] = rng.uniform(-1, 1, (6, d // 2)) * 9e-40
+    x = torch.from_numpy(x).to("cuda", ref.TORCH[dtype])
+    w = torch.ones(d, dtype=ref.TORCH[dtype], device="cuda")
+    s = torch.full((1,), 1e-41, device="cuda")
+    q, scales, total = rms(b200, x, w, static=s)
+    check_rms(x, w, 1e-6, q, scales, total, None, s)
+    assert int((q.abs() < 127).sum()) > d
+
+
 def test_rms_norm_ties(b200):
     """Products that lie exactly between two steps go to the even one: s w 254 / max is a whole odd number."""
     d = 64
