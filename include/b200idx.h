@@ -164,7 +164,8 @@ int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64
                                const float* static_scale, int8_t* q, int64_t ldq, float* scales, void* stream);
 /* The same as the way into an Int8Flat index (kind int8 only): the rows of n states on the index's device become
  * vectors of the index, or queries.  States and residual are n x dim(h) without gaps, ready when the call is
- * made; the calls return when they are done.  Rows of one index are comparable under INNER_PRODUCT and L2 when
+ * made; distances and labels lie on the index's device too (as may managed memory in any place); the calls return
+ * when they are done.  Rows of one index are comparable under INNER_PRODUCT and L2 when
  * they share a scale, so these metrics take a static_scale, the same for base and queries; INT8_COSINE, which
  * does not depend on it, also takes NULL (a scale per row). */
 int b200idx_add_states_device(b200idx_t* h, int64_t n, int dtype, const void* x, const void* residual, const void* weight,

@@ -43,14 +43,15 @@ struct Operand {
     const void* p;
     size_t align;
 };
-// Presence and alignment first (no device needed), then the device that holds all of them.
+constexpr int kAnyDevice = -1;   // of managed memory, which every device reaches
+// Presence and alignment first (no device needed), then the device that holds all of them, or kAnyDevice.
 int device_of(std::initializer_list<Operand> ops) {
     for (const Operand& o : ops) {
         if (!o.p) throw std::invalid_argument(std::string("Invalid ") + o.name + ": nullptr.");
         if (reinterpret_cast<uintptr_t>(o.p) % o.align != 0)
             throw std::invalid_argument(std::string(o.name) + " must be aligned to " + std::to_string(o.align) + " bytes");
     }
-    int device = -1;
+    int device = kAnyDevice;
     for (const Operand& o : ops) {
         cudaPointerAttributes at;
         const cudaError_t e = cudaPointerGetAttributes(&at, o.p);
@@ -63,11 +64,21 @@ int device_of(std::initializer_list<Operand> ops) {
             throw std::invalid_argument(std::string(o.name) + " must be a device pointer");
         }
         if (at.type == cudaMemoryTypeManaged) continue;
-        if (device >= 0 && at.device != device) throw std::invalid_argument("the pointers lie on different devices");
+        if (device != kAnyDevice && at.device != device) throw std::invalid_argument("the pointers lie on different devices");
         device = at.device;
     }
-    if (device < 0) cudaGetDevice(&device);
     return device;
+}
+// Where a call without an index runs: the operands' device, the current one where none is named.
+int device_for(std::initializer_list<Operand> ops) {
+    int device = device_of(ops);
+    if (device == kAnyDevice) B200_CUDA_CHECK(cudaGetDevice(&device));
+    return device;
+}
+// A call on an index runs on the index's device.
+void check_on(const FlatIndex* ix, std::initializer_list<Operand> ops, const char* what) {
+    const int device = device_of(ops);
+    if (device != kAnyDevice && device != ix->device()) throw std::invalid_argument(std::string(what) + " must lie on the index's device");
 }
 
 FlatIndex* states_index(b200idx_t* h) {
@@ -83,9 +94,8 @@ RmsNormArgs states_args(const FlatIndex* ix, int64_t n, int dtype, const void* x
     if (!static_scale && ix->metric() != kMetricCos)
         throw std::invalid_argument("inner products and L2 distances need a static_scale: rows with scales of their own do not compare");
     const Operand xo{"x", x, eb};
-    if (device_of({xo, {"weight", weight, eb}, residual ? Operand{"residual", residual, eb} : xo,
-                   static_scale ? Operand{"static_scale", static_scale, 4} : xo}) != ix->device())
-        throw std::invalid_argument("the states must lie on the index's device");
+    check_on(ix, {xo, {"weight", weight, eb}, residual ? Operand{"residual", residual, eb} : xo,
+                  static_scale ? Operand{"static_scale", static_scale, 4} : xo}, "the states");
     RmsNormArgs a{};
     a.x = x;
     a.ldx = a.ldr = ix->d();
@@ -122,7 +132,7 @@ int b200idx_rms_norm_i8_device(int64_t n, int d, int dtype, const void* x, int64
             throw std::invalid_argument("sum in place of x or residual needs the same stride");
         const float* sc = static_scale ? static_scale : scales;
         const Operand no{"q", q, 1};   // (repeats a required one where the optional ones are absent)
-        DeviceGuard g(device_of({{"x", x, eb}, {"weight", weight, eb}, no, {"scales", sc, 4},
+        DeviceGuard g(device_for({{"x", x, eb}, {"weight", weight, eb}, no, {"scales", sc, 4},
                                  residual ? Operand{"residual", residual, eb} : no, sum ? Operand{"sum", sum, eb} : no}));
         B200_CUDA_CHECK(launch_rms_norm_i8(dtype, a, static_cast<cudaStream_t>(stream)));
     });
@@ -146,7 +156,7 @@ int b200idx_search_states_device(b200idx_t* h, int64_t n, int dtype, const void*
         FlatIndex* ix = states_index(h);
         const RmsNormArgs a = states_args(ix, n, dtype, x, residual, weight, eps, static_scale);
         if (k <= 0 || k > 4096) throw std::invalid_argument("k must be > 0 and <= 4096");
-        device_of({{"distances", distances, 4}, {"labels", labels, 8}});
+        check_on(ix, {{"distances", distances, 4}, {"labels", labels, 8}}, "distances and labels");
         ix->search_states(n, dtype, a, k, distances, labels);
     });
 }
@@ -159,7 +169,7 @@ int b200idx_i8_dequantize_device(int64_t n, int d, const int8_t* q, int64_t ldq,
         const size_t eb = elem_bytes(dtype);
         if (!static_scale == !scales) throw std::invalid_argument("give exactly one of static_scale and scales");
         const int64_t lq = stride(ldq, d, "ldq"), lo = stride(ldo, d, "ldo");
-        DeviceGuard g(device_of({{"q", q, 1}, {"scales", scales ? scales : static_scale, 4}, {"out", out, eb}}));
+        DeviceGuard g(device_for({{"q", q, 1}, {"scales", scales ? scales : static_scale, 4}, {"out", out, eb}}));
         B200_CUDA_CHECK(launch_i8_dequantize(n, d, q, lq, scales, static_scale, dtype, out, lo, static_cast<cudaStream_t>(stream)));
     });
 }
@@ -172,8 +182,7 @@ int b200idx_scores_device(b200idx_t* h, int64_t n, const float* x, int dtype, vo
         check_rows(n, "n");
         const size_t eb = elem_bytes(dtype);
         if (ldo != 0 && ldo < ix->ntotal()) throw std::invalid_argument("ldo must be 0 or >= ntotal");
-        if (device_of({{"x", x, 4}, {"out", out, eb}}) != ix->device())
-            throw std::invalid_argument("x and out must lie on the index's device");
+        check_on(ix, {{"x", x, 4}, {"out", out, eb}}, "x and out");
         ix->scores_device(n, x, dtype, out, ldo ? ldo : ix->ntotal());
     });
 }
@@ -190,7 +199,7 @@ int b200idx_mx4_quantize_device(int64_t n, int d, int dtype, const void* x, int6
         check_dim(d);
         const size_t eb = elem_bytes(dtype);
         const int64_t lx = stride(ldx, d, "ldx");
-        DeviceGuard g(device_of({{"x", x, eb}, {"codes", codes, 16}, {"scales", scales, 16}}));
+        DeviceGuard g(device_for({{"x", x, eb}, {"codes", codes, 16}, {"scales", scales, 16}}));
         B200_CUDA_CHECK(launch_mx4_quantize(dtype, n, d, x, lx, 0, codes, scales, nullptr, static_cast<cudaStream_t>(stream)));
     });
 }
@@ -202,7 +211,7 @@ int b200idx_mx4_dequantize_device(int64_t n, int d, const uint8_t* codes, const 
         check_dim(d);
         const size_t eb = elem_bytes(dtype);
         const int64_t lo = stride(ldo, d, "ldo");
-        DeviceGuard g(device_of({{"codes", codes, 16}, {"scales", scales, 16}, {"out", out, eb}}));
+        DeviceGuard g(device_for({{"codes", codes, 16}, {"scales", scales, 16}, {"out", out, eb}}));
         B200_CUDA_CHECK(launch_mx4_dequantize(0, n, d, codes, scales, dtype, out, lo, static_cast<cudaStream_t>(stream)));
     });
 }
@@ -216,8 +225,8 @@ int b200idx_mx4_product_device(int64_t m, int64_t n, int d, const uint8_t* a_cod
         check_dim(d);
         const size_t eb = elem_bytes(dtype);
         if (ldo != 0 && ldo < n) throw std::invalid_argument("ldo must be 0 or >= n");
-        const int device = device_of({{"a_codes", a_codes, 16}, {"a_scales", a_scales, 16}, {"b_codes", b_codes, 16},
-                                      {"b_scales", b_scales, 16}, {"out", out, eb}});
+        const int device = device_for({{"a_codes", a_codes, 16}, {"a_scales", a_scales, 16}, {"b_codes", b_codes, 16},
+                                       {"b_scales", b_scales, 16}, {"out", out, eb}});
         DeviceGuard g(device);
         launch_mx4_product(dtype, Mx4ProductArgs{m, n, d, a_codes, a_scales, b_codes, b_scales, out, ldo ? ldo : n},
                            sm_count(device), static_cast<cudaStream_t>(stream));
