@@ -745,9 +745,11 @@ void FlatIndex::search_device(int64_t nq, const void* xq, bool q_is_f16, int k, 
                 B200_CUDA_CHECK(launch_gather_rows(mask_dev_, qmap + o0, m, static_cast<int>(mask_stride_ * 4), fm, stream_));
                 mask_cur_ = static_cast<const uint32_t*>(fm);
             }
-            run_tail(run_page(m, fq, fq, k, D, I, ldk, qmap + o0, true), false);
+            const PageTail tail = run_page(m, fq, fq, k, D, I, ldk, qmap + o0, true);
+            run_tail(tail, false);
             B200_CUDA_CHECK(cudaStreamSynchronize(stream_));
             timer_.collect(stats_);
+            throw_on_error(tail);
         }
     }
 }
