@@ -86,6 +86,10 @@ cudaError_t FlatIndex::launch_gemm(const GemmLaunch& L, const GemmArgs& a, const
     return launch_dist_gemm(L, a, map_a, &map_b_, stream_);
 }
 
+static void throw_wait(int err) {
+    if (err) throw std::runtime_error("device pipeline reported error word " + std::to_string(err) + " (bounded wait ran out)");
+}
+
 void FlatIndex::reserve(int64_t n) {
     if (n <= cap_rows_) return;
     // the rows move: what points at them is out of date even if an allocation below fails and the add with it
@@ -210,9 +214,12 @@ void FlatIndex::scores_device(int64_t nq, const float* xq, int out_dtype, void* 
     uint8_t* qop = static_cast<uint8_t*>(w_qop_.ensure(static_cast<size_t>(nq) * op_row_bytes()));
     uint8_t* qsc = static_cast<uint8_t*>(w_qsc_.ensure(static_cast<size_t>(mx4_scale_bytes(nq, d_))));
     B200_CUDA_CHECK(launch_mx4_quantize(kF32, nq, d_, xq, d_, 0, qop, qsc, nullptr, stream_));
-    launch_mx4_product(out_dtype, Mx4ProductArgs{nq, n_, d_, qop, qsc, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), out, ldo}, num_sms_, stream_);
+    int* err = static_cast<int*>(h_over_.ensure(sizeof(int)));
+    *err = 0;
+    launch_mx4_product(out_dtype, Mx4ProductArgs{nq, n_, d_, qop, qsc, xop_.as<uint8_t>(), xsc_.as<uint8_t>(), out, ldo, err}, num_sms_, stream_);
     stats_.kernel_launches += 2;
     B200_CUDA_CHECK(cudaStreamSynchronize(stream_));
+    throw_wait(*static_cast<volatile int*>(err));
 }
 
 size_t FlatIndex::mx4_file_row() const { return static_cast<size_t>(mx4_pitch(d_)) + mx4_blocks(d_); }
@@ -650,7 +657,7 @@ void FlatIndex::throw_on_error(const PageTail& t) {
     const int err = *t.e.err_host;
     if (!err) return;
     cudaMemsetAsync(w_err_.get(), 0, sizeof(int), stream_);
-    throw std::runtime_error("device pipeline reported error word " + std::to_string(err) + " (bounded wait ran out)");
+    throw_wait(err);
 }
 
 void FlatIndex::search_device(int64_t nq, const void* xq, bool q_is_f16, int k, float* D, int64_t* I, int ldk) {

@@ -19,6 +19,7 @@ struct Mx4ProductArgs {
     const uint8_t* b_scales;
     void* out;        // [m][ldo] in dtype
     int64_t ldo;
+    int* err = nullptr;   // gets kDevErrPipelineTimeout where a wait runs out (plain stores, so it may lie in pinned memory)
 };
 // throws where a launch fails; num_sms: of the current device
 void launch_mx4_product(int dtype, const Mx4ProductArgs& a, int num_sms, cudaStream_t stream);

@@ -62,6 +62,7 @@ struct ProductArgs {
     int64_t ldo;
     int a_tiles, b_tiles;    // tiles of TN rows of a, of 128 rows of b
     int split;               // CTAs of a cluster that share a tile's K (1: none)
+    int* err;                // where a wait that ran out is reported, or nullptr
     int b_first;             // mx4_few_kernel: first tile of b
     GemmArgs g;              // mx4_few_kernel as a pass of a search: thresholds and candidate lists
 };
@@ -99,6 +100,9 @@ __device__ __forceinline__ void store_columns(const uint32_t (&r)[COLS], const P
     }
 }
 
+__device__ __forceinline__ void report_abort(const ProductArgs& p) {
+    if (p.err && (threadIdx.x & 31) == 0) *reinterpret_cast<volatile int*>(p.err) = kDevErrPipelineTimeout;
+}
 // The end of a CTA: TMEM goes back; a split tile (bt, at), whose parts lie in shared memory as [TN][128], is added up.
 template <int THREADS, int TN, typename T>
 __device__ __forceinline__ void finish(const ProductArgs& p, bool owns_tmem, uint32_t tmem_base, volatile int& abort_flag, uint8_t* smem,
@@ -106,6 +110,7 @@ __device__ __forceinline__ void finish(const ProductArgs& p, bool owns_tmem, uin
     // After an abort, copies in flight get time to land before the shared memory is used again or released.
     __syncwarp();
     if (abort_flag) {
+        report_abort(p);
         const long long t0 = clock64();
         while (clock64() - t0 < 4000000LL) { }
     }
@@ -277,7 +282,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
                 // TN = 256: shared are 160 .. 255 of accumulator 0, 0 .. 95 of accumulator 1
                 if (lane == 0 && (TN != 256 || (ab ? group < 2 : group >= 2))) ptx::mbar_arrive(&bar_acc_free[TN == 256 ? 0 : ab]);
             } else {
-                // nobody reads an error word behind a product: results that could not be computed are no numbers
+                // whether somebody reads an error word or not: results that could not be computed are no numbers
 #pragma unroll
                 for (int c = 0; c < K::kCols; ++c) r[c] = 0x7fffffffu;
             }
@@ -582,6 +587,7 @@ void launch(const Mx4ProductArgs& q, int num_sms, cudaStream_t st) {
     p.n = q.n;
     p.out = q.out;
     p.ldo = q.ldo;
+    p.err = q.err;
     p.a_tiles = div_up(q.m, TN);
     p.b_tiles = div_up(q.n, kLanes);
     const int64_t total = static_cast<int64_t>(p.a_tiles) * p.b_tiles;
@@ -771,6 +777,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     // (after an abort, copies in flight get time to land; neither CTA's memory goes before both are done)
     __syncwarp();
     if (abort_flag) {
+        report_abort(p);
         const long long t0 = clock64();
         while (clock64() - t0 < 4000000LL) { }
     }
@@ -812,6 +819,7 @@ bool launch_pair(const Mx4ProductArgs& q, cudaStream_t st) {
     p.n = q.n;
     p.out = q.out;
     p.ldo = q.ldo;
+    p.err = q.err;
     p.split = 1;
     p.a_tiles = div_up(q.m, 256);
     p.b_tiles = div_up(q.n, 256);

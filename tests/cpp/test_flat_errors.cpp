@@ -38,9 +38,28 @@ static void searches_again(int dtype) {
     on_select = nullptr;
 }
 
+static void scores() {
+    constexpr int kN = 300, kD = 64;
+    FlatIndex ix(kD, kMetricIP, kMX4, 0);
+    std::vector<float> x(kN * kD), out(kN);
+    ix.add(kN, x.data(), false, nullptr, false);
+    bool late = false;
+    on_product = [&](const Mx4ProductArgs& a) {
+        if (late && a.err) *a.err = kDevErrPipelineTimeout;
+    };
+    auto call = [&] { return thrown([&] { ix.scores_device(1, x.data(), kF32, out.data(), kN); }); };
+    check(call().empty(), "scores");
+    late = true;
+    check(names_the_wait(call()), "the wait of a product of scores runs out: the call says so");
+    late = false;
+    check(call().empty(), "and the next does not");
+    on_product = nullptr;
+}
+
 int main() {
     searches_again(kMX4);
     searches_again(kF16);
+    scores();
     std::printf("%d failed\n", failed);
     return failed != 0;
 }
