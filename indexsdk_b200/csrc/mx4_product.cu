@@ -21,6 +21,7 @@
 #include <stdexcept>
 #include <type_traits>
 
+#include "cluster_limit.h"
 #include "ptx_sm100.cuh"
 #include "row_ops.cuh"
 #include "smem_limit.h"
@@ -805,11 +806,8 @@ bool launch_pair(const Mx4ProductArgs& q, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     // pairs that the device runs at a time (an odd number of SMs in a group leaves one without a partner)
-    static const int pairs = [&] {
-        int v = 0;
-        cfg.gridDim = dim3(2);
-        return cudaOccupancyMaxActiveClusters(&v, kern, &cfg) == cudaSuccess ? v : 0;
-    }();
+    cfg.gridDim = dim3(2);
+    const int pairs = clusters_at_once(reinterpret_cast<const void*>(kern), cfg);
     ProductArgs p{};
     p.a_scales = q.a_scales;
     p.b_scales = q.b_scales;

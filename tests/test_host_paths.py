@@ -11,6 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 @pytest.mark.parametrize("name, sources", [
     ("test_index_operands", ["ops_api.cu", "flat_index.cu"]),
     ("test_flat_errors", ["flat_index.cu"]),
+    ("test_cluster_limit", []),
 ])
 def test_host_paths(tmp_path, name, sources):
     exe = str(tmp_path / name)
