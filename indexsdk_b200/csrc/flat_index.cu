@@ -576,6 +576,10 @@ FlatIndex::PageTail FlatIndex::run_page(int nq, const void* xq_raw, const void* 
     t.e.I = I;
     t.e.ldk = ldk;
     t.e.qmap = qmap_dev;
+    // Up to 128 queries, sample and full pass are two kernels in which queries and base rows have changed sides
+    // (launch_mx4_few_search).  Nothing says that the tensor core rounds their sums alike, and no margin on a threshold
+    // bounds by how much it may not: a list that holds k keys holds the k best by its own sums, and any other is no result.
+    t.e.tau = dtype_ == kMX4 && plan.sampled ? tau : nullptr;
     // statuses and the error word: pinned memory that the last kernels write to, and only when there is
     // something to say (a copy and its launch cost 6 us each)
     t.status = static_cast<uint8_t*>(h_over_.ensure(static_cast<size_t>(nq) + sizeof(int) + 8));
@@ -733,8 +737,8 @@ void FlatIndex::search_device(int64_t nq, const void* xq, bool q_is_f16, int k, 
             if (tail.status[i]) over_idx.push_back(static_cast<int32_t>(q0 + i));
     }
     if (!over_idx.empty()) {
-        // Candidate overflow (heavy ties or an unrepresentative sample): re-run those queries
-        // with no threshold, every base row a candidate.
+        // Candidate overflow (heavy ties or an unrepresentative sample), or a list that came short of its threshold's
+        // promise (MX4): re-run those queries with no threshold, every base row a candidate.
         stats_.fallback_queries += over_idx.size();
         const int64_t n_pad = round_up(n_, kTileB);
         int64_t fpage = static_cast<int64_t>(kCandBudgetBytes / (static_cast<size_t>(n_pad) * 8));

@@ -445,6 +445,11 @@ select_emit_kernel(const uint64_t* cand, const uint32_t* counts, uint32_t n_fixe
         for (uint32_t i = threadIdx.x; i < k; i += NT) emit_one(e, q, static_cast<int>(i), kCandInvalid);
         return;
     }
+    auto fewer_than_k = [&] {
+        if (threadIdx.x || !e.tau || __ldg(e.tau + q) >= float_to_ord(__int_as_float(0x7f800000))) return;
+        if (overflow) overflow[q] = 1;
+        if (any_overflow) *any_overflow = 1u;
+    };
     uint64_t* sorted = sel_sm;
     uint64_t* held = sel_sm + P;
     const uint64_t* src = row;
@@ -455,6 +460,7 @@ select_emit_kernel(const uint64_t* cand, const uint32_t* counts, uint32_t n_fixe
             src = held;
         }
         if (m <= static_cast<uint32_t>(kSmallSet)) {
+            if (m < k) fewer_than_k();
             for (uint32_t i = threadIdx.x; i < m; i += NT) {
                 const uint64_t v = held[i];
                 uint32_t r = 0;
@@ -522,6 +528,7 @@ select_emit_kernel(const uint64_t* cand, const uint32_t* counts, uint32_t n_fixe
     const uint32_t found = block_kth32<NT>([&](auto&& f) { each([&](uint64_t v) { f(static_cast<uint32_t>(v >> 32)); }); },
                                            k, rank, 4);
     const bool enough = rank.n >= k;   // else all of them (rank.n is left as it was set)
+    if (!enough) fewer_than_k();
     if (enough) {
         kth = found;
         if (threadIdx.x == 0) {

@@ -70,11 +70,15 @@ struct EmitArgs {
     const int* err;          // device error word of the passes before, and where the host reads it (pinned, zeroed by
     int* err_host;           // the host beforehand); nullptr: the caller reads the word itself
     const MemberView* members;   // with q_mod: row q's labels are those of member q / q_mod (device array, or nullptr)
+    const uint32_t* tau;     // thresholds of lists that may be SHORT (launch_select_emit), or nullptr: at least k keys lie at
+                             // or below a finite threshold by the sums it was made from, but the keys in the list are another
+                             // kernel's sums, which may be rounded otherwise
 };
 // Per query: the k smallest of cand[q][0..min(counts[q],cap)) in ascending order as results (FLT_MAX / -1
 // where there are fewer).  counts == nullptr means every row holds n_fixed candidates.  overflow[q] is
 // set to 1 when counts[q] > cap (the row's results are then padding and the caller searches for the query
-// again, without a threshold), and so is *any_overflow; neither is written otherwise.  D, I, overflow and
+// again, without a threshold), or when e.tau is given, tau[q] finite and fewer than k candidates are there, and so is
+// *any_overflow; neither is written otherwise.  D, I, overflow and
 // any_overflow may lie in pinned host memory: stores there cost no copy and no wait of their own.
 cudaError_t launch_select_emit(const uint64_t* cand, const uint32_t* counts, uint32_t n_fixed, uint32_t cap,
                                uint8_t* overflow, uint32_t* any_overflow, const EmitArgs& e, cudaStream_t stream);

@@ -56,10 +56,30 @@ static void scores() {
     on_product = nullptr;
 }
 
+// The selection gets the thresholds where another kernel may have made them, and none where every row is a candidate.
+static void thresholds(int dtype, bool want) {
+    constexpr int kN = 70000, kD = 64;
+    FlatIndex ix(kD, kMetricL2, dtype, 0);
+    std::vector<float> x(static_cast<size_t>(kN) * kD), D(4);
+    std::vector<int64_t> I(4);
+    ix.add(kN, x.data(), false, nullptr, false);
+    int calls = 0;
+    on_select = [&](uint64_t*, const uint32_t* counts, uint32_t, uint8_t* over, const EmitArgs& e) {
+        ++calls;
+        check((e.tau != nullptr) == (want && counts != nullptr), "thresholds for the selection");
+        if (e.tau && over) over[0] = 1;   // (came short)
+    };
+    ix.search_device(1, x.data(), false, 4, D.data(), I.data(), 4);
+    check(calls == (want ? 2 : 1) && ix.stats().fallback_queries == (want ? 1u : 0u), "a short list is searched for again");
+    on_select = nullptr;
+}
+
 int main() {
     searches_again(kMX4);
     searches_again(kF16);
     scores();
+    thresholds(kMX4, true);
+    thresholds(kF16, false);
     std::printf("%d failed\n", failed);
     return failed != 0;
 }

@@ -2,6 +2,9 @@
 
 Rows and queries are normal values: blocks have scales of 2^-3 .. 2^0, products are multiples of 2^-8 and sums stay
 below |q| |x| < 2^13 for d <= 4096, so every fp32 sum is exact and distances and labels have to be equal."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 import torch
@@ -223,6 +226,56 @@ def test_refusals(b200):
     with pytest.raises(b200.B200IdxError) as e:
         ix.search_device_noalloc(d.data_ptr(), 2, 1, D.data_ptr(), I.data_ptr())
     assert e.value.code == 2001 and "MX4" in e.value.msg
+
+
+def test_lists_that_come_short(b200, tmp_path):
+    """Up to 128 queries, thresholds and candidates come from two kernels, which need not round alike."""
+    from indexsdk_b200 import build
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    objects = [os.path.join(build.BUILD_DIR, s[:-3] + ".o") for s in build.SOURCES]
+    if not all(map(os.path.exists, objects)):
+        build.build(force=True)
+    exe = str(tmp_path / "test_short_lists")
+    subprocess.run(["/usr/bin/g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), "-I", "/usr/local/cuda/include",
+                    os.path.join(root, "tests", "cpp", "test_short_lists.cpp"), *objects, "-o", exe,
+                    "-Wl,--wrap=_ZN4b20020launch_kth_thresholdEPKjiiiiPKfjPjRKNS_7TauFoldEP11CUstream_st",
+                    "-L/usr/local/cuda/lib64", "-lcudart_static", "-lpthread", "-ldl", "-lrt"], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "0 failed" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("metric", [0, 1])
+@pytest.mark.parametrize("n, nq, d, k", [(30000, 1, 128, 1), (30000, 64, 128, 20), (9000, 128, 1024, 100), (140001, 16, 64, 10),
+                                         (30000, 129, 256, 20)])
+def test_sums_that_round(b200, n, nq, d, k, metric):
+    """Scales spread over 2^24 in rows and in queries: fp32 holds no sum exactly.  A key is off by at most
+    2 eps d sum |q| |x| (half a step each of at most 2 d additions and cuts, relative to the largest partial sum), for L2
+    twice that and the roundings of two norms and two additions; so is the j-th smallest of the keys against the j-th
+    smallest of the exact ones, and so is the key of the row that a label names."""
+    rng = np.random.default_rng(n + d)
+
+    def wide(rows):
+        c, s = rng.integers(0, 16, (rows, d)), rng.integers(-12, 12, (rows, d // 32))
+        v = ref.MAGNITUDES[c & 7] * np.where(c & 8, -1.0, 1.0)
+        v[:, ::32] = 6.0   # (a block that holds its largest value keeps its scale)
+        return (v.reshape(rows, -1, 32) * np.exp2(s)[:, :, None]).reshape(rows, d)
+
+    x, q = wide(n), wide(nq)
+    ix = b200.IndexFlat(d, metric, b200.MX4)
+    ix.add(x.astype(np.float32))
+    np.testing.assert_array_equal(ix.get_base(), x)
+    D, I = ix.search(q.astype(np.float32), k)
+    assert I.min() >= 0 and all(len(set(r)) == k for r in I.tolist())
+    exact = ((q * q).sum(1)[:, None] + (x * x).sum(1) - 2 * q @ x.T) if metric == b200.METRIC_L2 else q @ x.T
+    bound = 2 * ref.EPS[0] * d * (np.abs(q) @ np.abs(x).T)
+    if metric == b200.METRIC_L2:
+        bound = 2 * bound + ref.EPS[0] * (d / 8 + 8) * ((q * q).sum(1)[:, None] + (x * x).sum(1))
+    worst = bound.max(1, keepdims=True)
+    best = np.sort(exact, 1)[:, :k] if metric == b200.METRIC_L2 else -np.sort(-exact, 1)[:, :k]
+    assert (np.abs(D - best) <= worst).all()
+    assert (np.abs(np.take_along_axis(exact, I, 1) - D) <= np.take_along_axis(bound, I, 1)).all()
+    step = np.diff(D, axis=1) if metric == b200.METRIC_L2 else -np.diff(D, axis=1)
+    assert (step >= 0).all()
 
 
 # ---- hidden states into an Int8Flat index ----
