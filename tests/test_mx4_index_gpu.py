@@ -278,6 +278,20 @@ def test_sums_that_round(b200, n, nq, d, k, metric):
     assert (step >= 0).all()
 
 
+def test_save_and_load_keeps_norms(b200, tmp_path):
+    """L2 distances of a loaded index, bit for bit: norms are sums that round here."""
+    rng = np.random.default_rng(7)
+    n, d = 700, 528
+    x = (rng.standard_normal((n, d)) * np.exp2(rng.integers(-12, 12, (n, d // 16))).repeat(16, 1)).astype(np.float32)
+    ix = b200.IndexFlat(d, b200.METRIC_L2, b200.MX4)
+    ix.add(x)
+    path = str(tmp_path / "mx4.b2ix")
+    ix.save(path)
+    again = b200.load_index(path)
+    for q in (x[:5], np.zeros((1, d), np.float32)):   # (distances from 0 are the norms themselves)
+        check(again.search(q, n), ix.search(q, n))
+
+
 # ---- hidden states into an Int8Flat index ----
 @pytest.mark.parametrize("metric, static", [(0, True), (1, True), (2, False), (2, True)])
 @pytest.mark.parametrize("residual", [False, True])

@@ -324,6 +324,21 @@ def test_i8_dequantize(b200, n, d, ldq, ldo, dtype):
     assert torch.equal(out[:, :d], (q[:, :d].float() * scales[0]).to(ref.TORCH[dtype]))
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("n, d", [(1, 9), (5, 9), (33, 77), (4, 777), (7, 1001), (1000, 13), (2001, 8), (3, 15), (130, 100)])
+def test_i8_dequantize_rows_without_gaps(b200, n, d, dtype):
+    """Rows that end inside a thread's eight outputs, which then have the scales of two rows; a last piece of fewer than eight."""
+    rng = np.random.default_rng(n + d)
+    q = torch.from_numpy(rng.integers(-128, 128, (n, d)).astype(np.int8)).cuda()
+    scales = torch.from_numpy(np.exp2(rng.integers(-3, 4, n)).astype(np.float32) * 1.25).cuda()
+    for given in (False, True):
+        out = torch.full((n * d + 16,), 3.0, dtype=ref.TORCH[dtype], device="cuda")
+        b200.i8_dequantize_device(n, d, q.data_ptr(), dtype, out.data_ptr(), scales_ptr=0 if given else scales.data_ptr(),
+                                  static_scale_ptr=scales.data_ptr() if given else 0, stream_ptr=_stream())
+        want = (q.float() * (scales[0] if given else scales[:, None])).to(ref.TORCH[dtype])
+        assert torch.equal(out[:n * d].view(n, d), want) and bool((out[n * d:] == 3.0).all())
+
+
 # ---- MX4 product ----
 def product(b, m, n, d, a, bb, dtype=0, ldo=0):
     out = torch.full((m * (ldo or n) + 16,), -3.0, dtype=ref.TORCH[dtype], device="cuda")
