@@ -825,31 +825,53 @@ cudaError_t rms_launch(const RmsNormArgs& a, cudaStream_t st) {
 }
 template <typename T, bool VEC, bool RES>
 cudaError_t rms_rows(const RmsNormArgs& a, cudaStream_t st) {
-    // Threads a row, chunks of 8 elements a thread, blocks an SM (which hold the registers down).  What carries the
-    // memory's rate is bytes on the way: 32 of x and 32 of the residual for each of 700 to 1000 threads of an SM, 64 of
-    // x alone.  65 536 x 4096 bf16, us: with residual 256 threads x 2, 3 blocks 308 (6.1 TB/s), 2 blocks 326, 128 x 4
-    // 313; without 256 x 2 240, 128 x 4 195.  fp32 with residual: 256 x 2, 3 blocks 566, 4 blocks (spills) 727.
-    // Rows off the 16-byte boundaries, one element a load: 8 elements a thread (60 000 x 1001 bf16 157 -> 123 us).
+    // Threads a row, chunks of 8 elements a thread, blocks an SM (which hold the registers down; forms that then spill were
+    // the faster ones all the same).  What carries the memory's rate is bytes on the way: 32 of x and 32 of the residual for
+    // each of 700 to 1000 threads of an SM, 64 of x alone.  A line ends where its threads hold no longer row; us of 2^27
+    // elements with this line / with the next one (threads x chunks / blocks where that is no neighbour), a scale per row:
+    //   16 bits, residual      d 128: 177 / 379; 256: 177 / 364; 512: 166 / 250; 768: 166 / 232; 1024: 158 / 361 (32 x 4 / 5: 181);
+    //                          2048: 160 / 373 (64 x 4 / 12: 191); 4096: 164 / 406 (128 x 4 / 6: 187); 8192: 179 / 392
+    //   16 bits, x alone       128: 128 (four blocks 130) / 285; 256: 132 / 259 (8 x 4 / 5: 138); 512: 117 / 177; 768: 115 / 148;
+    //                          1024: 105 (64 x 2 / 12: 117) / 234; 2048: 105 (128 x 2 / 6: 119) / 236;
+    //                          4096: 103 (256 x 2 / 3: 123) / 336; 8192: 170 / 291
+    //   rows off the 16-byte boundaries, one element a load, 16 bits:
+    //     residual             128: 411 (five blocks 440) / 592; 256: 332 / 534; 512: 281 (32 x 2 / 5: 414) / 519; 1001: 285
+    //                          (64 x 2 / 12: 338) / 568; 2048: 304 (128 x 2 / 6: 371) / 625; 4096: 353 (256 x 2 / 3: 404) / 637
+    //     x alone              128: 264 (five blocks 297) / 490; 256: 261 / 396; 512: 205 (32 x 2 / 5: 238) / 343; 600: 295
+    //                          (32 x 3 / 4: 473, 128 x 1 / 8: 324); 1001: 195 (128 x 1 / 8: 205) / 355; 2048: 201 (256 x 1 / 4:
+    //                          218) / 414; 4096: 222 (512 x 1 / 2: 263) / 435
+    //   fp32, residual         128: 342 / 652; 256: 302 / 537; 512: 312 / 451; 1024: 288 / 461; 2048: 283 / 485; 4096: 297 / 603;
+    //                          8192: 353 / 600
+    //   fp32, x alone          128: 226 / 523; 256: 226 / 334; 512: 166 / 328; 1024: 162 / 332; 2048: 168 / 349; 4096: 181 / 474;
+    //                          8192: 259 / 383
+    // One given scale (64-bit sums of squares) costs 16-bit rows 5 to 30 % more (4096, x alone: 103 -> 134), fp32 rows 2 to 7 with
+    // a residual and 8 to 22 without.
     if constexpr (sizeof(T) == 2 && !VEC) {
         if (a.d > 256 && a.d <= 512) return rms_launch<T, VEC, RES, 64, 1, 16>(a, st);
+    }
+    if constexpr (sizeof(T) == 2 && !VEC && RES) {
         if (a.d > 512 && a.d <= 1024) return rms_launch<T, VEC, RES, 128, 1, 8>(a, st);
         if (a.d > 1024 && a.d <= 2048) return rms_launch<T, VEC, RES, 256, 1, 4>(a, st);
         if (a.d > 2048 && a.d <= 4096) return rms_launch<T, VEC, RES, 512, 1, 2>(a, st);
     }
     if constexpr (sizeof(T) == 2 && VEC && !RES) {
-        if (a.d > 128 && a.d <= 256) return rms_launch<T, VEC, RES, 8, 4, 5>(a, st);
         if (a.d > 768 && a.d <= 1024) return rms_launch<T, VEC, RES, 32, 4, 5>(a, st);
         if (a.d > 1024 && a.d <= 2048) return rms_launch<T, VEC, RES, 64, 4, 12>(a, st);
         if (a.d > 2048 && a.d <= 4096) return rms_launch<T, VEC, RES, 128, 4, 6>(a, st);
     }
+    if constexpr (sizeof(T) == 2 && VEC) {
+        if (a.d > 256 && a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 5>(a, st);
+        if (a.d > 512 && a.d <= 768) return rms_launch<T, VEC, RES, 32, 3, 4>(a, st);
+    }
     if constexpr (sizeof(T) == 2) {
-        if (a.d <= 128) return rms_launch<T, VEC, RES, 8, 2, RES ? 4 : 5>(a, st);
+        if (a.d <= 128) return rms_launch<T, VEC, RES, 8, 2, VEC && !RES ? 5 : 4>(a, st);
         if (a.d <= 256) return rms_launch<T, VEC, RES, 16, 2, 4>(a, st);
-        if (a.d <= 512) return rms_launch<T, VEC, RES, 32, 2, 5>(a, st);
-        if (a.d <= 768) return rms_launch<T, VEC, RES, 32, 3, 4>(a, st);
-        if (a.d <= 1024) return rms_launch<T, VEC, RES, 64, 2, 12>(a, st);
-        if (a.d <= 2048) return rms_launch<T, VEC, RES, 128, 2, 6>(a, st);
-        if (a.d <= 4096) return rms_launch<T, VEC, RES, 256, 2, 3>(a, st);
+        // (what a line above takes for these is not built a second time)
+        if constexpr (VEC == RES) {
+            if (a.d <= 1024) return rms_launch<T, VEC, RES, 64, 2, 12>(a, st);
+            if (a.d <= 2048) return rms_launch<T, VEC, RES, 128, 2, 6>(a, st);
+            if (a.d <= 4096) return rms_launch<T, VEC, RES, 256, 2, 3>(a, st);
+        }
         if (a.d <= 8192) return rms_launch<T, VEC, RES, 512, 2, 2>(a, st);
         return rms_launch<T, VEC, RES, 512, 4>(a, st);
     } else {
