@@ -324,7 +324,7 @@ struct Few {
 constexpr int kNearAll = 2048;
 template <int TN>
 struct NearList {
-    static constexpr int kSlots = kNearAll / TN;
+    enum : int { kSlots = kNearAll / TN };
     uint32_t taken[TN];      // slots reserved, may pass kSlots
     uint32_t base[TN];
     float tau[TN];

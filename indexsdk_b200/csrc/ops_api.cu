@@ -1,5 +1,7 @@
 // extern "C" surface of the operators on rows in few bits (include/b200idx.h): argument checks, the device
-// the pointers live on, launches.  Nothing here allocates or waits, so calls can be captured into graphs.
+// the pointers live on, launches.  The calls without an index allocate nothing and wait for nothing, so they can be captured
+// into graphs; those on an index (states in and against one, all scores) use its scratch memory and its stream, and return
+// when they are done.
 #include "../../include/b200idx.h"
 
 #include <initializer_list>

@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(NT <= 32 ? 128 : NT, FIT) rms_norm_i8_kernel(c
             }
         } else {
             if (t == 0 && real) {
-                // the scale to the last bit of fp32, since the values that users take back carry its error: 1 / root by
-                // one step of Newton's method in 64 bits
+                // The values that users take back carry the scale's error, so it is rounded to fp32 once: 1 / root by one
+                // step of Newton's method in 64 bits.  What is left is the fp32 sum of eight squares in `part`, at most 4 steps of
+                // 2^-24 after the root (65 536 x 4096: one scale in 26 is not the nearest fp32 number, but the next).
                 const double ms = ssq / a.d + static_cast<double>(a.eps), r0 = rsqrtf(static_cast<float>(ms));
                 a.scales[row] = static_cast<float>(most * (r0 * (1.5 - 0.5 * ms * r0 * r0)) * (1. / 127.));
             }
@@ -431,40 +432,40 @@ __global__ void __launch_bounds__(256) i8_dequantize_kernel(uint32_t total, Divi
                                                             int64_t ldo) {
     const uint32_t step = gridDim.x * 256 * (FLAT ? 8 : 1);
     uint32_t i = (blockIdx.x * 256 + threadIdx.x) * (FLAT ? 8 : 1);
-    if (!FLAT) {
+    if constexpr (!FLAT) {
         for (; i < total; i += step) {
             const uint32_t row = by.quotient(i), k = i - row * by.d;
             const float s = __ldg(scales ? scales + row : static_scale);
             out[row * ldo + k] = from_f<T>(static_cast<float>(q[row * ldq + k]) * s);
         }
-        return;
-    }
-    for (; i < total; i += 2 * step) {   // two pieces at a time: their loads are on the way together
-        uint2 u[2];
-        float s[2], s2[2];
-        uint32_t first[2];   // elements that belong to the first row
+    } else {
+        for (; i < total; i += 2 * step) {   // two pieces at a time: their loads are on the way together
+            uint2 u[2];
+            float s[2], s2[2];
+            uint32_t first[2];   // elements that belong to the first row
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const uint32_t at = i + p * step;
-            if (at + 8 > total) continue;
-            const uint32_t row = by.quotient(at);
-            first[p] = by.d - (at - row * by.d);
-            u[p] = *reinterpret_cast<const uint2*>(q + at);
-            s[p] = __ldg(scales ? scales + row : static_scale);
-            s2[p] = first[p] < 8 && scales ? __ldg(scales + row + 1) : s[p];   // (d >= 8)
-        }
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t at = i + p * step;
+                if (at + 8 > total) continue;
+                const uint32_t row = by.quotient(at);
+                first[p] = by.d - (at - row * by.d);
+                u[p] = *reinterpret_cast<const uint2*>(q + at);
+                s[p] = __ldg(scales ? scales + row : static_scale);
+                s2[p] = first[p] < 8 && scales ? __ldg(scales + row + 1) : s[p];   // (d >= 8)
+            }
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const uint32_t at = i + p * step;
-            if (at + 8 <= total) {
-                float f[8];
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t at = i + p * step;
+                if (at + 8 <= total) {
+                    float f[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e)
-                    f[e] = static_cast<float>(static_cast<int8_t>((e < 4 ? u[p].x : u[p].y) >> (8 * (e & 3)))) * (e < first[p] ? s[p] : s2[p]);
-                store8<T>(out + at, f);
-            } else {
-                for (uint32_t e = at; e < total; ++e)
-                    out[e] = from_f<T>(static_cast<float>(q[e]) * __ldg(scales ? scales + by.quotient(e) : static_scale));
+                    for (uint32_t e = 0; e < 8; ++e)
+                        f[e] = static_cast<float>(static_cast<int8_t>((e < 4 ? u[p].x : u[p].y) >> (8 * (e & 3)))) * (e < first[p] ? s[p] : s2[p]);
+                    store8<T>(out + at, f);
+                } else {
+                    for (uint32_t e = at; e < total; ++e)
+                        out[e] = from_f<T>(static_cast<float>(q[e]) * __ldg(scales ? scales + by.quotient(e) : static_scale));
+                }
             }
         }
     }
@@ -925,9 +926,12 @@ template <typename T, int LOAD>
 cudaError_t mx4_round_rows(int64_t n, int d, const T* x, int64_t ldx, int64_t row0, uint8_t* codes, uint8_t* scales,
                            float* norms, cudaStream_t st) {
     const T* end = x + (n - 1) * ldx + d;
-    if (norms) {
-        mx4_quantize_norms_kernel<T, LOAD><<<warp_blocks(n), 256, 0, st>>>(n, d, x, ldx, end, row0, codes, scales, norms);
-        return cudaGetLastError();
+    if (norms) {   // (rows and queries of an index, which are fp32)
+        if constexpr (std::is_same<T, float>::value) {
+            mx4_quantize_norms_kernel<T, LOAD><<<warp_blocks(n), 256, 0, st>>>(n, d, x, ldx, end, row0, codes, scales, norms);
+            return cudaGetLastError();
+        }
+        return cudaErrorInvalidValue;
     }
     const int ng = mx4_groups(d);
     return by_stretches(n, ng, [&](int64_t r, int64_t m) {

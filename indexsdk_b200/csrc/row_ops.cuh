@@ -40,7 +40,7 @@ cudaError_t launch_rms_norm_i8(int dtype, const RmsNormArgs& a, cudaStream_t str
 cudaError_t launch_i8_dequantize(int64_t n, int d, const int8_t* q, int64_t ldq, const float* scales,
                                  const float* static_scale, int dtype, void* out, int64_t ldo, cudaStream_t stream);
 
-// codes / scales: the whole buffers; the n rows of x become rows row0, row0 + 1, ...  norms: nullptr or an fp32
+// codes / scales: the whole buffers; the n rows of x become rows row0, row0 + 1, ...  norms: nullptr or (kF32 only) an fp32
 // array indexed like the rows, which gets the squared norms of the ROUNDED rows.
 cudaError_t launch_mx4_quantize(int dtype, int64_t n, int d, const void* x, int64_t ldx, int64_t row0, uint8_t* codes,
                                 uint8_t* scales, float* norms, cudaStream_t stream);
