@@ -288,7 +288,7 @@ typedef struct {
     uint64_t stage_launches[B200IDX_NUM_STAGES];
     uint64_t searches;
     uint64_t queries;
-    uint64_t fallback_queries; /* queries re-run without a threshold after a candidate overflow (IVFPQ: exact re-scan) */
+    uint64_t fallback_queries; /* queries re-run without a threshold: candidate lists that overflowed or came short (IVFPQ: exact re-scan) */
     uint64_t gemm_launches;
     uint64_t kernel_launches;  /* kernels of this library launched by searches */
     uint64_t scan_codes;       /* IVFPQ: PQ codes visited so far */
